@@ -420,6 +420,36 @@ int nemo_mask_weight(const int32_t* object_idx, const int32_t* source_vert_idx, 
                      const int32_t* verts_end, const float* verts_dist_weight, float weight_x, float weight_c,
                      int32_t clutter_start, int32_t S, int32_t K, int32_t V, float* out, void* stream);
 
+/* ---- the contrastive loss of the feature bank: products, log probabilities, gradients ---------------------------
+ * The loss over the bank (softmax of similarity / T - weight over the bank's rows, cross entropy at the slot's own row:
+ * what the reference's training step computes from FeatureBankNeMo's similarity and MaskCreater's weights,
+ * nemo/models/nemo.py:138-209, nemo/models/feature_banks.py:39-232) and the dense layer in front of it.  Rows may be
+ * strided (a row stride `ld*` in elements, elements of a row contiguous); outputs are contiguous.  Element types: */
+#define NEMO_F32  0
+#define NEMO_BF16 1
+#define NEMO_F16  2
+/* y[M,N] = act(alpha x[M,K] weight[N,K]^T + bias[N]) + beta residual[M,N].  All tensors of one element type; products are
+ * summed in f32 and the result is rounded once.  activation: 0 none, 1 relu, 2 gelu (with erf), 3 silu.  bias, residual
+ * may be NULL.  pre [M,N] or NULL: alpha x W^T + bias in the element type, what nemo_linear_backward needs when there is an
+ * activation.  K = 0 gives act(bias) + beta residual.  workspace: nemo_linear_workspace bytes of device memory
+ * (asked with the same pointers and strides: operands whose rows are not aligned to 16 bytes are copied into it), contents
+ * undefined before and after. */
+size_t nemo_linear_workspace(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K, int32_t dtype);
+int nemo_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation, float alpha, float beta, void* y, void* pre,
+                void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of the above from grad_y [M,N]: with dz = grad_y act'(pre),
+ *   grad_x = alpha dz W, grad_weight = alpha dz^T x, grad_bias = column sums of dz, grad_residual = beta grad_y.
+ * Any output may be NULL (not wanted); operands that only unwanted outputs need may be NULL too.  dz is rounded to the
+ * element type in front of the two products (they run on the matrix cores); the column sums take it unrounded.  Sums run in a
+ * fixed order: two calls give the same bits. */
+size_t nemo_linear_backward_workspace(const void* grad_y, int64_t ldg, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                      int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation);
+int nemo_linear_backward(const void* grad_y, int64_t ldg, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                         const void* pre, int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation, float alpha, float beta,
+                         void* grad_x, void* grad_weight, void* grad_bias, void* grad_residual, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

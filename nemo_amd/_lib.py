@@ -23,6 +23,7 @@ SYMBOLS = [
     "nemo_solve", "nemo_keypoint_corr", "nemo_solve_flow", "nemo_spherical_angles",
     "nemo_solve_features_workspace", "nemo_solve_features_supported", "nemo_solve_features", "nemo_render_nearest", "nemo_raster_forms",
     "nemo_project_keypoints", "nemo_gather_features", "nemo_gather_features_backward", "nemo_gather_idx", "nemo_mask_weight",
+    "nemo_linear_workspace", "nemo_linear", "nemo_linear_backward_workspace", "nemo_linear_backward",
 ]
 
 
@@ -109,12 +110,19 @@ def load():
     lib.nemo_gather_features_backward.argtypes = [f32p, f32p, f32p, f32p, vp, i32, i32, i32, f32p, f32p, vp]
     lib.nemo_gather_idx.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp]
     lib.nemo_mask_weight.argtypes = [vp, vp, vp, vp, f32p, C.c_float, C.c_float, i32, i32, i32, i32, f32p, vp]
+    i64, sz = C.c_int64, C.c_size_t
+    lib.nemo_linear_workspace.argtypes = [vp, i64, vp, i64, i64, i64, i64, i32]
+    lib.nemo_linear_backward_workspace.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, i32]
+    lib.nemo_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, i32, i32, C.c_float, C.c_float, vp, vp, vp, sz, vp]
+    lib.nemo_linear_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i32, i32, C.c_float, C.c_float, vp, vp, vp, vp, vp, sz, vp]
+    for name in ("nemo_linear_workspace", "nemo_linear_backward_workspace"):
+        getattr(lib, name).restype = sz
     for name in SYMBOLS:
         fn = getattr(lib, name)
         if name not in ("nemo_last_error", "nemo_version", "nemo_grid_score_workspace", "nemo_similarity_table_elems",
                         "nemo_grid_pack_bytes", "nemo_grid_score_packed_workspace", "nemo_grid_score_recentred_workspace", "nemo_grid_fragments_bytes",
                         "nemo_grid_score_fragments_workspace", "nemo_vertex_similarity_workspace",
-                        "nemo_solve_features_workspace"):
+                        "nemo_solve_features_workspace", "nemo_linear_workspace", "nemo_linear_backward_workspace"):
             fn.restype = C.c_int
     _lib = lib
     return lib

@@ -1,0 +1,80 @@
+// What the dense operators (linear.hip, log_probs.hip, bank_log_probs.hip) share: element types, matrix-core fragments, the
+// direct copy from global memory to LDS, reductions.
+//
+// A fragment is 16 bytes a lane, for either operand of a product:
+//   16-bit types  v_mfma_f32_16x16x32: lane = (row r = lane % 16, group g = lane / 16), elements k = 8 g .. 8 g + 7 of a block of 32;
+//   f32           v_mfma_f32_32x32x2 (four of them): lane = (row r = lane % 32, group g = lane / 32), elements k = 4 g .. 4 g + 3 of a
+//                 block of 8.  The hardware pairs element i of one operand with element i of the other; which k that is does not
+//                 matter as long as both operands agree, so four consecutive f32 are loaded at once.
+// Results: lane % FR is the row of the SECOND operand (q); the FIRST operand's rows (p) run through the registers, four consecutive
+// ones at a time: register 4 b + i holds p = 8 b + 4 (lane / 32) + i (f32) or 4 (lane / 16) + i (16-bit types).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace nemo {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+#define NEMO_LDS __attribute__((address_space(3)))
+#define NEMO_GLOBAL __attribute__((address_space(1)))
+
+template <typename T> __device__ inline float to_f32(T x) { return (float)x; }
+template <typename T> __device__ inline T from_f32(float x) { return (T)x; }       // round to nearest even
+
+__device__ inline float neg_inf() { return -__builtin_inff(); }
+
+// ---- matrix cores ---------------------------------------------------------------------------------------------------------------
+template <typename T> struct Mma;
+
+template <> struct Mma<float> {
+    typedef f32x16_t Acc;
+    static constexpr int FR = 32, NG = 2, KF = 8, QUADS = 4;           // rows of a fragment, lane groups, k of a fragment, p quads of a result
+    static __device__ inline void run(Acc& acc, const u32x4& p, const u32x4& q) {
+        const f32x4 a = __builtin_bit_cast(f32x4, p), b = __builtin_bit_cast(f32x4, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
+    }
+};
+
+template <> struct Mma<bf16> {
+    typedef f32x4 Acc;
+    static constexpr int FR = 16, NG = 4, KF = 32, QUADS = 1;
+    static __device__ inline void run(Acc& acc, const u32x4& p, const u32x4& q) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), acc, 0, 0, 0);
+    }
+};
+
+template <> struct Mma<f16> {
+    typedef f32x4 Acc;
+    static constexpr int FR = 16, NG = 4, KF = 32, QUADS = 1;
+    static __device__ inline void run(Acc& acc, const u32x4& p, const u32x4& q) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, p), __builtin_bit_cast(f16x8_t, q), acc, 0, 0, 0);
+    }
+};
+
+// 64 lanes copy 16 bytes each from their own global addresses to 1024 consecutive bytes of LDS at `lds` (the same for all lanes).
+__device__ inline void copy_to_lds(const void* g, void* lds) {
+    __builtin_amdgcn_global_load_lds((NEMO_GLOBAL void*)g, (NEMO_LDS void*)lds, 16, 0, 0);
+}
+
+// ---- reductions -----------------------------------------------------------------------------------------------------------------
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ inline float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+}  // namespace nemo

@@ -25,6 +25,7 @@
 #include <utility>
 
 #include "../../include/nemo_hip.h"
+#include "errors.h"
 #include "raster.h"
 #include "resample.h"
 
@@ -37,21 +38,13 @@ using namespace nemo;
 // ------------------------------------------------------------------------------------------
 static thread_local char g_err[512] = "";
 
-static int fail(int code, const char* fmt, ...) {
+int nemo::fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
     return code;
 }
-
-#define HIP_TRY(expr)                                                                         \
-    do {                                                                                      \
-        hipError_t e_ = (expr);                                                               \
-        if (e_ != hipSuccess)                                                                 \
-            return fail(NEMO_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), \
-                        __FILE__, __LINE__);                                                  \
-    } while (0)
 
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 

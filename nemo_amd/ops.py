@@ -687,3 +687,75 @@ def spherical_angles(campos):
     with torch.cuda.device(cp.device):
         check(lib.nemo_spherical_angles(ptr(cp), cp.shape[0], ptr(out), stream_ptr()), "nemo_spherical_angles")
     return out
+
+
+# ---- the contrastive loss of the feature bank (contrastive.py adds autograd and the checks of its arguments) ----
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def rows_2d(t, width):
+    """(t as [rows, width] whose rows are contiguous, row stride in elements): a view where the strides allow it, else a copy.
+    Rows may lie apart (a slice of wider rows); overlapping or permuted ones are copied."""
+    t = t.detach()
+    if t.dim() != 2:
+        rows = 1
+        for n in t.shape[:-1]:
+            rows *= n
+        t = t.reshape(rows, width)
+    if t.is_contiguous() or t.numel() == 0:
+        return t, width
+    if (width == 1 or t.stride(1) == 1) and t.stride(0) >= width:
+        return t, t.stride(0)
+    return t.contiguous(), width
+
+
+def _raw(t):
+    return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _scratch(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, beta=1.0, want_pre=False):
+    """-> (y [M,N], pre [M,N] or None): y = act(alpha x weight^T + bias) + beta residual; x [M,K], weight [N,K] of one type."""
+    lib = _lib.load()
+    (M, K), N = x.shape, weight.shape[0]
+    x, ldx = rows_2d(x, K)
+    weight, ldw = rows_2d(weight, K)
+    ldr = N
+    if residual is not None:
+        residual, ldr = rows_2d(residual, N)
+    if bias is not None:
+        bias = bias.detach().contiguous()
+    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    pre = torch.empty(M, N, dtype=x.dtype, device=x.device) if want_pre else None
+    dt = DTYPES[x.dtype]
+    with torch.cuda.device(x.device):
+        nbytes = lib.nemo_linear_workspace(_raw(x), ldx, _raw(weight), ldw, M, N, K, dt)
+        ws = _scratch(nbytes, x.device)
+        check(lib.nemo_linear(_raw(x), ldx, _raw(weight), ldw, _raw(bias), _raw(residual), ldr, M, N, K, dt, ACTIVATIONS[activation],
+                              float(alpha), float(beta), _raw(y), _raw(pre), _raw(ws), nbytes, stream_ptr()), "nemo_linear")
+    return y, pre
+
+
+def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1.0, want=(True, True, False, False)):
+    """-> (grad_x, grad_weight, grad_bias, grad_residual), None where `want` is false.  x is only read for grad_weight and weight only
+    for grad_x: either may be its shape instead."""
+    lib = _lib.load()
+    (M, K), (N, _) = (t.shape if torch.is_tensor(t) else t for t in (x, weight))
+    x, ldx = rows_2d(x, K) if torch.is_tensor(x) else (None, K)
+    weight, ldw = rows_2d(weight, K) if torch.is_tensor(weight) else (None, K)
+    grad_y, ldg = rows_2d(grad_y, N)
+    dev, dt = grad_y.device, DTYPES[grad_y.dtype]
+    shapes = ((M, K), (N, K), (N,), (M, N))
+    empty = torch.zeros if M == 0 or N == 0 else torch.empty                # a sum over nothing is zero
+    outs = [empty(s, dtype=grad_y.dtype, device=dev) if w else None for s, w in zip(shapes, want)]
+    with torch.cuda.device(dev):
+        nbytes = lib.nemo_linear_backward_workspace(_raw(grad_y), ldg, _raw(x), ldx, _raw(weight), ldw, M, N, K, dt, ACTIVATIONS[activation])
+        ws = _scratch(nbytes, dev)
+        check(lib.nemo_linear_backward(_raw(grad_y), ldg, _raw(x), ldx, _raw(weight), ldw, _raw(pre), M, N, K, dt, ACTIVATIONS[activation],
+                                       float(alpha), float(beta), *[_raw(o) for o in outs], _raw(ws), nbytes, stream_ptr()),
+              "nemo_linear_backward")
+    return tuple(outs)
