@@ -450,6 +450,27 @@ int nemo_linear_backward(const void* grad_y, int64_t ldg, const void* x, int64_t
                          void* grad_x, void* grad_weight, void* grad_bias, void* grad_residual, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* Log probabilities of given places of rows of logits [rows,cols] (element type dtype, row stride ld):
+ *   z[i,j] = scale logits[i,j] - weights[i,j]   (two rounded f32 operations; a weight of +inf leaves the place out: z = -inf whatever
+ *                                                the logit is, and no gradient; weights f32, NULL, or with ldw = 0 one row for all),
+ *   lse[i] = log sum_j exp z[i,j],  p = exp(z - lse),  logp[i] = z[i,targets[i]] - lse[i],  entropy[i] = - sum_j p log p,
+ *   top_logp / top_index [rows,top]: the `top` (0..16) largest z of a row in descending order, the lowest place first among equal ones,
+ *   as log probabilities and places.
+ * targets[i] = -1: no target, logp 0; any other target outside 0..cols-1: logp NaN.  A row with nothing left (all z = -inf, or cols = 0):
+ * lse = -inf, entropy 0, logp -inf, no gradient.  A row with a NaN or +inf among its z: NaN outputs, top_index -1.  Missing best
+ * entries: top_logp -inf, top_index -1.  All outputs f32 (top_index i64); any may be NULL (top_* when top = 0).  out_stats [rows,4], on
+ * 16 bytes: what nemo_log_probs_backward needs.  workspace: nemo_log_probs_workspace bytes, contents undefined before and after. */
+size_t nemo_log_probs_workspace(int64_t rows, int64_t cols, int32_t top);
+int nemo_log_probs(const void* logits, int64_t ld, const float* weights, int64_t ldw, const int64_t* targets, int64_t rows, int64_t cols,
+                   int32_t dtype, float scale, int32_t top, float* out_logp, float* out_entropy, float* out_lse, float* out_stats,
+                   float* out_top_logp, int64_t* out_top_index, void* workspace, size_t workspace_bytes, void* stream);
+/* grad_logits [rows,cols] (contiguous, element type dtype) from the gradients of logp, entropy and lse (each [rows] f32 or NULL):
+ *   scale (p (g_lse - g_logp - g_entropy (log p + entropy)) + [j = target] g_logp), 0 where z = -inf.
+ * Rows whose target is outside -1..cols-1 get NaN. */
+int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights, int64_t ldw, const int64_t* targets, const float* stats,
+                            const float* g_logp, const float* g_entropy, const float* g_lse, int64_t rows, int64_t cols, int32_t dtype,
+                            float scale, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -93,3 +93,70 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
         M *= n
     y = _Linear.apply(x.reshape(M, K), weight, bias, None if residual is None else residual.reshape(M, N), activation, alpha, beta)
     return y.reshape(lead + (N,))
+
+
+LogProbs = namedtuple("LogProbs", "logp entropy lse top_logp top_index")
+
+
+def _probs_arguments(what, rows, cols, device, targets, weights, scale, top):
+    """Checks what log_probs and bank_log_probs share -> (targets as i64, scale, top)."""
+    if not torch.is_tensor(targets) or targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: targets must be an int64 or int32 tensor")
+    if tuple(targets.shape) != (rows,):
+        raise ValueError(f"{what}: targets must be [{rows}], got {tuple(targets.shape)}")
+    if targets.device != device:
+        if targets.is_cuda:
+            raise RuntimeError(f"{what}: targets are on {targets.device}, the rows on {device}")
+        if targets.numel() and (int(targets.min()) < -1 or int(targets.max()) >= cols):      # on the host: nothing to wait for
+            raise ValueError(f"{what}: targets must lie in -1 .. {cols - 1}")
+    if weights is not None:
+        _device_tensors(what, (torch.float32,), weights=weights)
+        if weights.device != device:
+            raise RuntimeError(f"{what}: weights are on {weights.device}, the rows on {device}")
+        if tuple(weights.shape) not in ((cols,), (rows, cols)):
+            raise ValueError(f"{what}: weights must be [{cols}] or [{rows}, {cols}], got {tuple(weights.shape)}")
+        if weights.requires_grad:
+            raise ValueError(f"{what}: weights are constants, they get no gradient: pass weights.detach()")
+    if isinstance(top, bool) or int(top) != top or not 0 <= top <= 16:
+        raise ValueError(f"{what}: top must be a whole number in 0 .. 16, got {top}")
+    return targets.to(device=device, dtype=torch.int64), _number(what, "scale", scale), int(top)
+
+
+class _LogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, weights, scale, top):
+        out, stats, top_logp, top_index = ops.log_probs(logits, targets, weights, scale, top)
+        ctx.save_for_backward(logits, targets, weights, stats)
+        ctx.scale = scale
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_index)
+        ctx.set_materialize_grads(False)
+        return out[0], out[1], out[2], top_logp, top_index
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_lse, *_):
+        logits, targets, weights, stats = ctx.saved_tensors
+        if g_logp is None and g_entropy is None and g_lse is None:
+            return None, None, None, None, None
+        return ops.log_probs_backward(logits, targets, weights, stats, g_logp, g_entropy, g_lse, ctx.scale), None, None, None, None
+
+
+def log_probs(logits, targets, weights=None, scale=1.0, top=0):
+    """Log probabilities of one place of every row of logits [S, V] under softmax(z), z = scale logits - weights.
+
+    -> LogProbs(logp [S] of the targets, entropy [S], lse [S] = log sum exp z, top_logp [S, top], top_index [S, top]), statistics in
+    float32 whatever the logits' type (float32, bfloat16, float16); top_logp and top_index (int64) are the `top` most probable places in
+    descending order, the lowest place first among equal ones (None, None for top = 0; they carry no gradient).
+
+    targets [S] int64 or int32: the place, or -1 for a row without a target (logp 0, no gradient through it).  Other values outside the row
+    are refused where the tensor is on the host and give NaN in that row (values and gradient) where it is on the device, which is not read
+    back.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place out, whatever the logit there is (NaN
+    too).  A row with nothing left: lse and logp -inf, entropy 0, top_index -1, gradient 0.  A row with a NaN or +inf left: NaN,
+    top_index -1.  Fewer places left than `top`: -inf and -1 in their stead."""
+    _device_tensors("log_probs", tuple(ops.DTYPES), logits=logits)
+    if logits.dim() != 2:
+        raise ValueError(f"log_probs: logits must be [S, V], got {tuple(logits.shape)}")
+    S, V = logits.shape
+    targets, scale, top = _probs_arguments("log_probs", S, V, logits.device, targets, weights, scale, top)
+    return LogProbs(*_LogProbs.apply(logits, targets, weights, scale, top))

@@ -1,0 +1,345 @@
+// Log probabilities of given places of rows of logits, with entropy, log-sum-exp and the best entries; and the gradient of the logits.
+//
+// Both directions read each logit once and are bound by memory.  Forward: a wave or a workgroup of four waves takes a row (or one of its
+// parts), a lane takes 16 bytes at a time and keeps the state of softmax_state.h; states are joined across lanes, waves and parts in a
+// fixed order.  For the best entries a lane keeps its best one; a wave takes the best of its lanes k times, and the lane it came from
+// looks through its share of the row again for the next one, together with the whole wave.  Waves' lists, sorted, are merged.
+// Rows need not be aligned: 16-byte accesses at any element are in order on this hardware.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/nemo_hip.h"
+#include "errors.h"
+#include "softmax_state.h"
+
+namespace nemo {
+
+struct LogProbArgs {
+    const void* logits;
+    long ld;
+    const float* weights;          // null, or rows with stride ldw (0: one row for all)
+    long ldw;
+    const long long* targets;
+    long rows;
+    int cols;
+    float scale;
+    int parts, part_cols;          // columns of a part, whole chunks
+    float* part_state;             // [3][parts][rows]
+    float* part_z;                 // [parts][rows][top]
+    int* part_place;
+    RowOut out;
+};
+
+template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T); T v[N]; };
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) LooseChunk { u32x4 v; };
+
+// Scores of up to N places from column j on; places at or beyond `end` are -inf.
+template <typename T>
+__device__ inline void chunk_scores(const T* row, const float* w, float scale, int j, int end, float z[Chunk<T>::N]) {
+    constexpr int N = Chunk<T>::N;
+    if (j + N <= end) {
+        union { u32x4 u; T t[N]; } c;
+        c.u = ((const LooseChunk<T>*)(row + j))->v;
+        if (w) {
+            float wv[N];
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) {
+                const u32x4 u = ((const LooseChunk<float>*)(w + j + 4 * q))->v;
+                const f32x4 f = __builtin_bit_cast(f32x4, u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) wv[4 * q + i] = f[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = score(to_f32(c.t[i]), scale, wv[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = score(to_f32(c.t[i]), scale);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            z[i] = j + i >= end ? neg_inf() : w ? score(to_f32(row[j + i]), scale, w[j + i]) : score(to_f32(row[j + i]), scale);
+    }
+}
+
+// A chunk's scores into a state: one rescaling a chunk.
+template <int N>
+__device__ inline void add_scores(SoftmaxState& a, const float z[N]) {
+    float m = a.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
+    const float d = a.m - m, f = fast_exp(d);
+    a.t = f * (a.t + fmaxf(d, -200.0f) * a.s);
+    a.s *= f;
+    a.m = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float dz = z[i] - m, e = fast_exp(dz);
+        a.s += e;
+        a.t += weighted(e, dz);
+    }
+}
+
+// WAVES waves a row, ROWS rows a workgroup (WAVES * ROWS = 4).
+template <typename T, int WAVES, bool TOP>
+__global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
+    constexpr int N = Chunk<T>::N, ROWS = 4 / WAVES, LANES = 64 * WAVES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int part = (int)(blockIdx.x % a.parts);
+    const long row = (long)(blockIdx.x / a.parts) * ROWS + wave / WAVES;
+    const bool live = row < a.rows;                                    // all four waves of a workgroup meet at the barriers below
+    const int wr = wave % WAVES;
+    const int begin = part * a.part_cols, end = min(a.cols, begin + a.part_cols);
+    const T* logits = (const T*)a.logits + (live ? row : 0) * a.ld;
+    const float* w = a.weights ? a.weights + (live ? row : 0) * a.ldw : nullptr;
+    const int first = begin + (wr * 64 + lane) * N;
+    SoftmaxState st = empty_state();
+    Entry best = no_entry();
+    if (live) {
+#pragma unroll 2
+        for (int j = first; j < end; j += LANES * N) {
+            float z[N];
+            chunk_scores<T>(logits, w, a.scale, j, end, z);
+            add_scores<N>(st, z);
+            if (TOP) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (z[i] > best.z) best = {z[i], j + i};           // places rise within a lane: the first of equal ones stays
+            }
+        }
+    }
+    st = wave_join(st);
+    __shared__ SoftmaxState s_state[4];
+    __shared__ Entry s_top[TOP ? 4 : 1][kMaxTop];
+    const int top = a.out.top;
+    if (TOP && live) {
+        for (int i = 0; i < top; ++i) {
+            const Entry e = wave_best(best);
+            if (lane == 0) s_top[wave][i] = e;
+            if (i + 1 == top || e.z == neg_inf()) {
+                if (lane == 0)
+                    for (int r = i + 1; r < top; ++r) s_top[wave][r] = no_entry();
+                break;
+            }
+            // the owner's share again: the best entry behind e
+            const int owner = ((e.place - begin) / N) & 63;
+            Entry next = no_entry();
+            for (int j = begin + (wr * 64 + owner) * N + lane * LANES * N; j < end; j += 64 * LANES * N) {
+                float z[N];
+                chunk_scores<T>(logits, w, a.scale, j, end, z);
+#pragma unroll
+                for (int q = 0; q < N; ++q) {
+                    const Entry c = {z[q], j + q};
+                    if (ahead(e, c) && ahead(c, next)) next = c;
+                }
+            }
+            next = wave_best(next);
+            if (lane == owner) best = next;
+        }
+    }
+    if (WAVES > 1) {
+        if (lane == 0) s_state[wave] = st;
+        __syncthreads();
+        if (wr != 0 || !live) return;
+        st = s_state[wave];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) st = join_states(st, s_state[wave + i]);
+    } else {
+        if (TOP) __syncthreads();
+        if (!live) return;
+    }
+    // the wave that is left merges the waves' lists: lane i < WAVES walks list i
+    if (a.parts > 1) {
+        const size_t at = (size_t)part * a.rows + row, plane = (size_t)a.parts * a.rows;
+        if (lane == 0) {
+            a.part_state[at] = st.m;
+            a.part_state[plane + at] = st.s;
+            a.part_state[2 * plane + at] = st.t;
+        }
+    } else if (lane == 0) {
+        const long long t = a.targets[row];
+        float zt = 0.0f;
+        if (t >= 0 && t < a.cols) zt = w ? score(to_f32(logits[t]), a.scale, w[t]) : score(to_f32(logits[t]), a.scale);
+        write_row(a.out, row, st, t, a.cols, zt);
+    }
+    if (TOP) {
+        int walk = 0;
+        for (int i = 0; i < top; ++i) {
+            const Entry mine = lane < WAVES && walk < top ? s_top[wave + lane][walk] : no_entry();
+            const Entry e = wave_best(mine);
+            if (mine.place == e.place && mine.z == e.z) ++walk;
+            if (lane == 0) {
+                if (a.parts > 1) {
+                    const size_t at = ((size_t)part * a.rows + row) * top + i;
+                    a.part_z[at] = e.z;
+                    a.part_place[at] = e.place;
+                } else {
+                    write_top(a.out, row, i, st, e);
+                }
+            }
+        }
+    }
+}
+
+// Joins the parts of a row (at most 64): a wave a row, a lane a part.
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const size_t at = (size_t)lane * a.rows + row, plane = (size_t)a.parts * a.rows;
+    SoftmaxState st = empty_state();
+    if (lane < a.parts) st = {a.part_state[at], a.part_state[plane + at], a.part_state[2 * plane + at]};
+    st = wave_join(st);
+    if (lane == 0) {
+        const long long t = a.targets[row];
+        float zt = 0.0f;
+        if (t >= 0 && t < a.cols) {
+            const float x = to_f32(((const T*)a.logits)[row * a.ld + t]);
+            zt = a.weights ? score(x, a.scale, a.weights[row * a.ldw + t]) : score(x, a.scale);
+        }
+        write_row(a.out, row, st, t, a.cols, zt);
+    }
+    int walk = 0;
+    for (int i = 0; i < a.out.top; ++i) {
+        Entry mine = no_entry();
+        if (lane < a.parts && walk < a.out.top) mine = {a.part_z[at * a.out.top + walk], a.part_place[at * a.out.top + walk]};
+        const Entry e = wave_best(mine);
+        if (mine.place == e.place && mine.z == e.z) ++walk;
+        if (lane == 0) write_top(a.out, row, i, st, e);
+    }
+}
+
+// d logits: 256 threads x 16 bytes a step of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_backward_kernel(LogProbArgs a, const float* stats, const float* g_logp, const float* g_entropy,
+                                                                 const float* g_lse, T* grad) {
+    constexpr int N = Chunk<T>::N;
+    for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const RowCoef k = row_coef(stats, g_logp, g_entropy, g_lse, a.targets, row, a.cols);
+        const T* logits = (const T*)a.logits + row * a.ld;
+        const float* w = a.weights ? a.weights + row * a.ldw : nullptr;
+        T* out = grad + row * (long)a.cols;
+#pragma unroll 2
+        for (int j = (blockIdx.x * 256 + threadIdx.x) * N; j < a.cols; j += gridDim.x * 256 * N) {
+            float z[N];
+            chunk_scores<T>(logits, w, a.scale, j, a.cols, z);
+            union { u32x4 u; T t[N]; } c;
+#pragma unroll
+            for (int i = 0; i < N; ++i) c.t[i] = from_f32<T>(a.scale * score_gradient(k, z[i], j + i));
+            if (j + N <= a.cols) {
+                ((LooseChunk<T>*)(out + j))->v = c.u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (j + i < a.cols) out[j + i] = c.t[i];
+            }
+        }
+    }
+}
+
+static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Parts of a row where there are too few rows to fill the device: four workgroups a compute unit, at least 8192 columns a part.
+static int parts_of(int64_t rows, int64_t cols) {
+    int64_t p = rows > 0 ? 1024 / rows : 1;
+    if (p > cols / 8192) p = cols / 8192;
+    return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
+}
+
+static int check_log_probs(const char* who, int64_t rows, int64_t cols, int dtype, int top) {
+    if (rows < 0 || cols < 0) return fail(NEMO_ERR_INVALID, "%s: negative size", who);
+    if (dtype != NEMO_F32 && dtype != NEMO_BF16 && dtype != NEMO_F16) return fail(NEMO_ERR_INVALID, "%s: unknown element type %d", who, dtype);
+    if (top < 0 || top > kMaxTop) return fail(NEMO_ERR_UNSUPPORTED, "%s: %d best entries (takes 0 to %d)", who, top, kMaxTop);
+    if (rows >= (1LL << 24) || cols > (1LL << 30)) return fail(NEMO_ERR_UNSUPPORTED, "%s: more than 2^24 - 1 rows or 2^30 columns", who);
+    return NEMO_OK;
+}
+
+template <typename T>
+static void launch_log_probs(const LogProbArgs& a, hipStream_t st) {
+    // One wave a row where a row is short and there are enough of them to fill the device that way; four waves a row otherwise.
+    const bool narrow = a.cols <= 2048 && a.rows >= 2048;
+    const unsigned wgs = narrow ? (unsigned)((a.rows + 3) / 4) : (unsigned)(a.rows * a.parts);
+    if (a.out.top) {
+        if (narrow) hipLaunchKernelGGL((log_probs_kernel<T, 1, true>), dim3(wgs), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((log_probs_kernel<T, 4, true>), dim3(wgs), dim3(256), 0, st, a);
+    } else {
+        if (narrow) hipLaunchKernelGGL((log_probs_kernel<T, 1, false>), dim3(wgs), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((log_probs_kernel<T, 4, false>), dim3(wgs), dim3(256), 0, st, a);
+    }
+    if (a.parts > 1) hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+}
+
+}  // namespace nemo
+
+using namespace nemo;
+
+extern "C" size_t nemo_log_probs_workspace(int64_t rows, int64_t cols, int32_t top) {
+    const int parts = parts_of(rows, cols);
+    if (rows <= 0 || parts <= 1) return 0;
+    return align256((size_t)3 * parts * rows * 4) + align256((size_t)parts * rows * top * 4) * 2;
+}
+
+extern "C" int nemo_log_probs(const void* logits, int64_t ld, const float* weights, int64_t ldw, const int64_t* targets, int64_t rows,
+                              int64_t cols, int32_t dtype, float scale, int32_t top, float* out_logp, float* out_entropy, float* out_lse,
+                              float* out_stats, float* out_top_logp, int64_t* out_top_index, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    int rc = check_log_probs("nemo_log_probs", rows, cols, dtype, top);
+    if (rc) return rc;
+    if (rows == 0) return NEMO_OK;
+    if (!targets || (cols > 0 && !logits) || (top > 0 && (!out_top_logp || !out_top_index)))
+        return fail(NEMO_ERR_INVALID, "nemo_log_probs: null argument");
+    if (ld < cols || (weights && ldw != 0 && ldw < cols)) return fail(NEMO_ERR_INVALID, "nemo_log_probs: a row stride shorter than the row");
+    if ((uintptr_t)out_stats & 15) return fail(NEMO_ERR_INVALID, "nemo_log_probs: out_stats must start on 16 bytes");
+    const size_t need = nemo_log_probs_workspace(rows, cols, top);
+    if (workspace_bytes < need || (need && !workspace))
+        return fail(NEMO_ERR_INVALID, "nemo_log_probs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    LogProbArgs a = {};
+    a.logits = logits; a.ld = ld; a.weights = weights; a.ldw = ldw; a.targets = (const long long*)targets;
+    a.rows = rows; a.cols = (int)cols; a.scale = scale;
+    a.parts = parts_of(rows, cols);
+    a.part_cols = (int)(((cols + a.parts - 1) / a.parts + 7) / 8 * 8);
+    if (a.parts > 1) {
+        char* ws = (char*)workspace;
+        a.part_state = (float*)ws;
+        ws += align256((size_t)3 * a.parts * rows * 4);
+        a.part_z = (float*)ws;
+        a.part_place = (int*)(ws + align256((size_t)a.parts * rows * top * 4));
+    }
+    a.out = {out_logp, out_entropy, out_lse, out_stats, out_top_logp, (long long*)out_top_index, top};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == NEMO_F32) launch_log_probs<float>(a, st);
+    else if (dtype == NEMO_BF16) launch_log_probs<bf16>(a, st);
+    else launch_log_probs<f16>(a, st);
+    HIP_TRY(hipGetLastError());
+    return NEMO_OK;
+}
+
+template <typename T>
+static void launch_log_probs_backward(const LogProbArgs& a, const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse,
+                                      void* grad, hipStream_t st) {
+    const int per = 256 * Chunk<T>::N;
+    const int slabs = (a.cols + 2 * per - 1) / (2 * per);              // two steps a thread
+    hipLaunchKernelGGL((log_probs_backward_kernel<T>), dim3(slabs, (unsigned)(a.rows < 65535 ? a.rows : 65535)), dim3(256), 0, st, a, stats, g_logp,
+                       g_entropy, g_lse, (T*)grad);
+}
+
+extern "C" int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights, int64_t ldw, const int64_t* targets,
+                                       const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse, int64_t rows,
+                                       int64_t cols, int32_t dtype, float scale, void* grad_logits, void* stream) {
+    int rc = check_log_probs("nemo_log_probs_backward", rows, cols, dtype, 0);
+    if (rc) return rc;
+    if (rows == 0 || cols == 0) return NEMO_OK;
+    if (!logits || !targets || !stats || !grad_logits) return fail(NEMO_ERR_INVALID, "nemo_log_probs_backward: null argument");
+    if (ld < cols || (weights && ldw != 0 && ldw < cols)) return fail(NEMO_ERR_INVALID, "nemo_log_probs_backward: a row stride shorter than the row");
+    if ((uintptr_t)stats & 15) return fail(NEMO_ERR_INVALID, "nemo_log_probs_backward: stats must start on 16 bytes");
+    LogProbArgs a = {};
+    a.logits = logits; a.ld = ld; a.weights = weights; a.ldw = ldw; a.targets = (const long long*)targets;
+    a.rows = rows; a.cols = (int)cols; a.scale = scale; a.parts = 1;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == NEMO_F32) launch_log_probs_backward<float>(a, stats, g_logp, g_entropy, g_lse, grad_logits, st);
+    else if (dtype == NEMO_BF16) launch_log_probs_backward<bf16>(a, stats, g_logp, g_entropy, g_lse, grad_logits, st);
+    else launch_log_probs_backward<f16>(a, stats, g_logp, g_entropy, g_lse, grad_logits, st);
+    HIP_TRY(hipGetLastError());
+    return NEMO_OK;
+}

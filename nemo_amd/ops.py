@@ -759,3 +759,54 @@ def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1
                                        float(alpha), float(beta), *[_raw(o) for o in outs], _raw(ws), nbytes, stream_ptr()),
               "nemo_linear_backward")
     return tuple(outs)
+
+
+def _row_weights(weights, cols):
+    """(tensor, row stride) of log-prob weights: None, one row for all ([cols], stride 0) or a row each."""
+    if weights is None:
+        return None, 0
+    if weights.dim() == 1:
+        return weights.detach().contiguous(), 0
+    return rows_2d(weights, cols)
+
+
+def _log_probs_outputs(rows, top, device):
+    out = torch.empty(3, rows, device=device)
+    stats = torch.empty(rows, 4, device=device)
+    top_logp = torch.empty(rows, top, device=device) if top else None
+    top_index = torch.empty(rows, top, dtype=torch.int64, device=device) if top else None
+    return out, stats, top_logp, top_index
+
+
+def log_probs(logits, targets, weights=None, scale=1.0, top=0):
+    """logits [S,V], targets [S] i64, weights None / [V] / [S,V] f32 -> (out [3,S] = logp, entropy, lse; stats [S,4] for the backward
+    call; top_logp [S,top], top_index [S,top] i64, or None, None)."""
+    lib = _lib.load()
+    S, V = logits.shape
+    logits, ld = rows_2d(logits, V)
+    weights, ldw = _row_weights(weights, V)
+    targets = targets.contiguous()
+    dev = logits.device
+    out, stats, top_logp, top_index = _log_probs_outputs(S, top, dev)
+    with torch.cuda.device(dev):
+        nbytes = lib.nemo_log_probs_workspace(S, V, top)
+        ws = _scratch(nbytes, dev)
+        check(lib.nemo_log_probs(_raw(logits), ld, _raw(weights), ldw, _raw(targets), S, V, DTYPES[logits.dtype], float(scale), int(top),
+                                 _raw(out[0]), _raw(out[1]), _raw(out[2]), _raw(stats), _raw(top_logp), _raw(top_index), _raw(ws), nbytes,
+                                 stream_ptr()), "nemo_log_probs")
+    return out, stats, top_logp, top_index
+
+
+def log_probs_backward(logits, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0):
+    """-> grad_logits [S,V] in the type of the logits; the gradients are [S] f32 or None."""
+    lib = _lib.load()
+    S, V = logits.shape
+    logits, ld = rows_2d(logits, V)
+    weights, ldw = _row_weights(weights, V)
+    targets = targets.contiguous()
+    gs = [None if g is None else g.detach().to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_lse)]
+    grad = torch.empty(S, V, dtype=logits.dtype, device=logits.device)
+    with torch.cuda.device(logits.device):
+        check(lib.nemo_log_probs_backward(_raw(logits), ld, _raw(weights), ldw, _raw(targets), _raw(stats), *[_raw(g) for g in gs], S, V,
+                                          DTYPES[logits.dtype], float(scale), _raw(grad), stream_ptr()), "nemo_log_probs_backward")
+    return grad
