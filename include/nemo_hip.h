@@ -471,6 +471,28 @@ int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights
                             const float* g_logp, const float* g_entropy, const float* g_lse, int64_t rows, int64_t cols, int32_t dtype,
                             float scale, void* grad_logits, void* stream);
 
+/* nemo_log_probs straight from features [rows,channels] and bank [cols,channels] (f32 or bf16, both the same):
+ *   z[i,j] = scale <features[i], bank[j]> - weights[i,j],
+ * same outputs and rules, the [rows,cols] matrix is never written.  Products are summed in f32 (f32: on the f32 matrix cores).  channels
+ * 1..256 (padded to 32, 64, 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same
+ * pointers and strides (rows that do not start on 16 bytes are copied into it), contents undefined before and after. */
+size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
+                                     int64_t channels, int32_t dtype, int32_t top);
+int nemo_bank_log_probs(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,
+                        const int64_t* targets, int64_t rows, int64_t cols, int64_t channels, int32_t dtype, float scale, int32_t top,
+                        float* out_logp, float* out_entropy, float* out_lse, float* out_stats, float* out_top_logp, int64_t* out_top_index,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* With dz as nemo_log_probs_backward has it (without its factor scale):
+ *   grad_features[i] = scale sum_j dz[i,j] bank[j],   grad_bank[j] = scale sum_i dz[i,j] features[i]
+ * (contiguous, element type dtype; NULL: not wanted).  The scores are computed again.  Places that are left out add nothing, whatever the
+ * feature or bank row holds.  Sums run in a fixed order: two calls give the same bits. */
+size_t nemo_bank_log_probs_backward_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
+                                              int64_t channels, int32_t dtype);
+int nemo_bank_log_probs_backward(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,
+                                 const int64_t* targets, const float* stats, const float* g_logp, const float* g_entropy,
+                                 const float* g_lse, int64_t rows, int64_t cols, int64_t channels, int32_t dtype, float scale,
+                                 void* grad_features, void* grad_bank, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

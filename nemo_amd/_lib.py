@@ -25,6 +25,7 @@ SYMBOLS = [
     "nemo_project_keypoints", "nemo_gather_features", "nemo_gather_features_backward", "nemo_gather_idx", "nemo_mask_weight",
     "nemo_linear_workspace", "nemo_linear", "nemo_linear_backward_workspace", "nemo_linear_backward",
     "nemo_log_probs_workspace", "nemo_log_probs", "nemo_log_probs_backward",
+    "nemo_bank_log_probs_workspace", "nemo_bank_log_probs", "nemo_bank_log_probs_backward_workspace", "nemo_bank_log_probs_backward",
 ]
 
 
@@ -119,14 +120,21 @@ def load():
     lib.nemo_log_probs_workspace.argtypes = [i64, i64, i32]
     lib.nemo_log_probs.argtypes = [vp, i64, vp, i64, vp, i64, i64, i32, C.c_float, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.nemo_log_probs_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i32, C.c_float, vp, vp]
-    for name in ("nemo_linear_workspace", "nemo_linear_backward_workspace", "nemo_log_probs_workspace"):
+    lib.nemo_bank_log_probs_workspace.argtypes = [vp, i64, vp, i64, i64, i64, i64, i32, i32]
+    lib.nemo_bank_log_probs.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i32, C.c_float, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.nemo_bank_log_probs_backward_workspace.argtypes = [vp, i64, vp, i64, i64, i64, i64, i32]
+    lib.nemo_bank_log_probs_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, C.c_float, vp, vp, vp, sz,
+                                                 vp]
+    dense_workspaces = ("nemo_linear_workspace", "nemo_linear_backward_workspace", "nemo_log_probs_workspace", "nemo_bank_log_probs_workspace",
+                        "nemo_bank_log_probs_backward_workspace")
+    for name in dense_workspaces:
         getattr(lib, name).restype = sz
     for name in SYMBOLS:
         fn = getattr(lib, name)
         if name not in ("nemo_last_error", "nemo_version", "nemo_grid_score_workspace", "nemo_similarity_table_elems",
                         "nemo_grid_pack_bytes", "nemo_grid_score_packed_workspace", "nemo_grid_score_recentred_workspace", "nemo_grid_fragments_bytes",
                         "nemo_grid_score_fragments_workspace", "nemo_vertex_similarity_workspace",
-                        "nemo_solve_features_workspace", "nemo_linear_workspace", "nemo_linear_backward_workspace", "nemo_log_probs_workspace"):
+                        "nemo_solve_features_workspace", *dense_workspaces):
             fn.restype = C.c_int
     _lib = lib
     return lib

@@ -160,3 +160,39 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0):
     S, V = logits.shape
     targets, scale, top = _probs_arguments("log_probs", S, V, logits.device, targets, weights, scale, top)
     return LogProbs(*_LogProbs.apply(logits, targets, weights, scale, top))
+
+
+class _BankLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, features, bank, targets, weights, scale, top):
+        out, stats, top_logp, top_index = ops.bank_log_probs(features, bank, targets, weights, scale, top)
+        ctx.save_for_backward(features, bank, targets, weights, stats)
+        ctx.scale = scale
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_index)
+        ctx.set_materialize_grads(False)
+        return out[0], out[1], out[2], top_logp, top_index
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_lse, *_):
+        features, bank, targets, weights, stats = ctx.saved_tensors
+        if g_logp is None and g_entropy is None and g_lse is None:
+            return (None,) * 6
+        grads = ops.bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, ctx.scale,
+                                            ctx.needs_input_grad[:2])
+        return (*grads, None, None, None, None)
+
+
+def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
+    """log_probs(linear(features, bank), ...) without the [S, V] matrix: features [S, C] and bank [V, C], both float32 or both bfloat16, C up
+    to 256.  Scores are z = scale <feature, bank row> - weights, summed in 32 bits; arguments, results and rules are those of log_probs.
+    Differentiable with respect to features and bank; the gradient computes the scores again instead of keeping them."""
+    _device_tensors("bank_log_probs", (torch.float32, torch.bfloat16), features=features, bank=bank)
+    if features.dim() != 2 or bank.dim() != 2 or features.shape[1] != bank.shape[1]:
+        raise ValueError(f"bank_log_probs: features must be [S, C] and bank [V, C], got {tuple(features.shape)} and {tuple(bank.shape)}")
+    if not 1 <= features.shape[1] <= 256:
+        raise ValueError(f"bank_log_probs: {features.shape[1]} channels (takes 1 to 256: use linear and log_probs)")
+    S, V = features.shape[0], bank.shape[0]
+    targets, scale, top = _probs_arguments("bank_log_probs", S, V, features.device, targets, weights, scale, top)
+    return LogProbs(*_BankLogProbs.apply(features, bank, targets, weights, scale, top))

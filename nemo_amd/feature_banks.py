@@ -7,7 +7,9 @@ it, the layout cu_layers/CuNeMo/gather_features.py:31 assumes).  `mesh_offsets` 
 give the pose solver what it needs.  Constructor signature, attribute names and the return values of forward /
 __call__ are the reference's (they are the drop-in boundary); the bodies are written for this package: the
 clutter ring buffer is a slice assignment, the weight matrices come from one `torch.where`, and the multi-class
-gather runs on the HIP replacement of the reference's CuNeMo extension (cu_nemo.gather_features / get_mask).
+gather runs on the HIP replacement of the reference's CuNeMo extension (cu_nemo.gather_features / get_mask).  `logits` and
+`log_probs` are the contrastive loss that the reference's training step computes from them (nemo/models/nemo.py:138-209), on the kernels
+of contrastive.py.
 """
 import math
 
@@ -15,6 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import contrastive
 from .cu_nemo import gather_features, get_mask
 
 _DEFAULT_KAPPAS = {"pos": 0, "near": 1e5, "clutter": 5, "class": 1e5}
@@ -173,6 +176,20 @@ class FeatureBankNeMo(nn.Module):
         buf = self.memory_neg.clone()
         buf[start:start + fits] = new[:fits]
         self.memory_neg = buf
+
+    # ---- the contrastive loss ----
+    def logits(self, feats, weights=None, T=1.0):
+        """similarity / T - weights of slots [S, C] with every bank row, [S, V_total + clutter rows], differentiable with respect to the
+        slots (and to weights): the logits of the reference's cross entropy.  weights: MaskCreater's rows or None."""
+        return contrastive.linear(feats, self.memory.to(feats.dtype), residual=weights, alpha=1.0 / T, beta=-1.0)
+
+    def log_probs(self, feats, rows, weights=None, T=1.0, top=0):
+        """Log probabilities of the slots' own bank rows (MaskCreater's second result; -1: none) under softmax(similarity / T - weights), with
+        entropy, log-sum-exp and the `top` most probable bank rows: contrastive.LogProbs.  The loss is -result.logp.mean().  No
+        [S, V_total + clutter rows] matrix is written for float32 and bfloat16 slots of up to 256 channels; others go through `logits`."""
+        if feats.dtype in (torch.float32, torch.bfloat16) and feats.shape[-1] <= 256:
+            return contrastive.bank_log_probs(feats, self.memory.to(feats.dtype), rows, weights=weights, scale=1.0 / T, top=top)
+        return contrastive.log_probs(contrastive.linear(feats, self.memory.to(feats.dtype), alpha=1.0 / T), rows, weights=weights, top=top)
 
     def forward(self, x, visible, x_to_bank=None, object_labels=None, vis_mask=None):
         """x [B, K (+ num_noise), C] vertex (+ clutter) features, visible [B, K].

@@ -810,3 +810,43 @@ def log_probs_backward(logits, targets, weights, stats, g_logp, g_entropy, g_lse
         check(lib.nemo_log_probs_backward(_raw(logits), ld, _raw(weights), ldw, _raw(targets), _raw(stats), *[_raw(g) for g in gs], S, V,
                                           DTYPES[logits.dtype], float(scale), _raw(grad), stream_ptr()), "nemo_log_probs_backward")
     return grad
+
+
+def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
+    """log_probs of scale features bank^T - weights without that matrix: features [S,C], bank [V,C] of one type.  Returns as log_probs."""
+    lib = _lib.load()
+    (S, ch), V = features.shape, bank.shape[0]
+    features, ldf = rows_2d(features, ch)
+    bank, ldb = rows_2d(bank, ch)
+    weights, ldw = _row_weights(weights, V)
+    targets = targets.contiguous()
+    dev, dt = features.device, DTYPES[features.dtype]
+    out, stats, top_logp, top_index = _log_probs_outputs(S, top, dev)
+    with torch.cuda.device(dev):
+        nbytes = lib.nemo_bank_log_probs_workspace(_raw(features), ldf, _raw(bank), ldb, S, V, ch, dt, top)
+        ws = _scratch(nbytes, dev)
+        check(lib.nemo_bank_log_probs(_raw(features), ldf, _raw(bank), ldb, _raw(weights), ldw, _raw(targets), S, V, ch, dt, float(scale),
+                                      int(top), _raw(out[0]), _raw(out[1]), _raw(out[2]), _raw(stats), _raw(top_logp), _raw(top_index),
+                                      _raw(ws), nbytes, stream_ptr()), "nemo_bank_log_probs")
+    return out, stats, top_logp, top_index
+
+
+def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0, want=(True, True)):
+    """-> (grad_features, grad_bank), None where `want` is false."""
+    lib = _lib.load()
+    (S, ch), V = features.shape, bank.shape[0]
+    features, ldf = rows_2d(features, ch)
+    bank, ldb = rows_2d(bank, ch)
+    weights, ldw = _row_weights(weights, V)
+    targets = targets.contiguous()
+    dev, dt = features.device, DTYPES[features.dtype]
+    gs = [None if g is None else g.detach().to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_lse)]
+    empty = torch.zeros if S == 0 or V == 0 else torch.empty
+    grads = [empty(n, ch, dtype=features.dtype, device=dev) if w else None for n, w in zip((S, V), want)]
+    with torch.cuda.device(dev):
+        nbytes = lib.nemo_bank_log_probs_backward_workspace(_raw(features), ldf, _raw(bank), ldb, S, V, ch, dt)
+        ws = _scratch(nbytes, dev)
+        check(lib.nemo_bank_log_probs_backward(_raw(features), ldf, _raw(bank), ldb, _raw(weights), ldw, _raw(targets), _raw(stats),
+                                               *[_raw(g) for g in gs], S, V, ch, dt, float(scale), *[_raw(g) for g in grads], _raw(ws),
+                                               nbytes, stream_ptr()), "nemo_bank_log_probs_backward")
+    return tuple(grads)
