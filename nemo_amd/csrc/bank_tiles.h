@@ -1,0 +1,140 @@
+// What the kernels of bank_log_probs.hip and bank_gradient.hip share: arguments, tiles in LDS, the first product.
+//
+// 32 "owner" rows, whose fragments a wave keeps in registers, are multiplied with tiles of "other" rows that the workgroup's four waves share in
+// LDS (two buffers, copied from global memory without registers), on v_mfma_f32_32x32x{16 bf16, 2 f32} with the other rows as first operand.
+// Register 4 b + i of lane l then holds the product of owner row l % 32 with other row 8 b + 4 (l / 32) + i: a lane sees one owner row only.
+#pragma once
+#include <type_traits>
+
+#include "softmax_state.h"
+
+namespace nemo {
+
+static __device__ const u32x4 g_zero_row = {0, 0, 0, 0};
+
+template <typename T> struct Wide;                                     // 32 x 32 products; a fragment is 16 bytes a lane
+template <> struct Wide<float> {
+    static constexpr int KF = 8;                                       // k of a fragment: group g holds 4 g .. 4 g + 3
+    static __device__ inline void run(f32x16_t& acc, const u32x4& p, const u32x4& q) { Mma<float>::run(acc, p, q); }
+};
+template <> struct Wide<bf16> {
+    static constexpr int KF = 16;                                      // group g holds 8 g .. 8 g + 7
+    static __device__ inline void run(f32x16_t& acc, const u32x4& p, const u32x4& q) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), acc, 0, 0, 0);
+    }
+};
+
+struct BankArgs {
+    const void* own;               // rows whose fragments stay in registers
+    const void* other;
+    long ld_own, ld_other;         // elements
+    int n_own, n_other, channels;
+    const float* weights;          // [features][ldw] or one row (ldw = 0) or null
+    long ldw;
+    const long long* targets;
+    float scale;
+    int parts, part_tiles;         // tiles of other rows a part
+    // forward
+    float* part_state;             // [3][2 parts][rows]
+    float* part_z;                 // [2 parts][rows][top]: products (scores where out.k = 0) in the order of their scores
+    int* part_place;
+    float* z_target;               // [rows]
+    RowOut out;
+    // backward
+    const float* coef;             // [K_COUNT][features]
+    float* partial;                // [parts][n_own][CP] when parts > 1
+    void* grad;                    // [n_own][channels]
+};
+
+// A tile in LDS.  Each instruction of a copy writes 1024 bytes, RPI rows; rows of 256 bytes and more get 16 RPI bytes of padding behind them, and
+// chunk c of row r lies at c ^ flip(r) within its row: rows that one LDS read touches at the same chunk then lie in different banks.  flip
+// reaches the lowest bits of a chunk index only, so that the addresses of a lane differ by constants, which need no registers.
+template <typename T, int CP> struct Tile {
+    static constexpr int RB = CP * (int)sizeof(T), CPR = RB / 16, RPI = 1024 / RB, PITCH = 1024 + (RB >= 256 ? 16 * RPI : 0);
+    static constexpr int MASK = RPI >= 16 ? 3 : RPI - 1;               // chunk bits that flip reaches
+    static constexpr int ROWS = RB >= 1024 ? 32 : 64;                  // rows of a tile
+    static constexpr int BYTES = ROWS / RPI * PITCH;
+    static __device__ constexpr int flip(int r) { return RPI >= 16 ? (r >> 1) & 3 : r & MASK; }
+    static __device__ constexpr int row(int r) { return r / RPI * PITCH + r % RPI * RB; }
+};
+
+template <typename T, int CP>
+__device__ inline void stage_rows(char* lds, const T* base, long ld, int row0, int rows, int channels, int wave, int lane) {
+    typedef Tile<T, CP> L;
+    constexpr int EPC = 16 / (int)sizeof(T);
+    static_assert(L::ROWS / L::RPI % 4 == 0, "every wave copies the same number of kilobytes");
+#pragma unroll
+    for (int i = 0; i < L::ROWS / L::RPI / 4; ++i) {
+        const int j = i * 4 + wave;
+        const int r = j * L::RPI + lane / L::CPR, c = (lane & (L::CPR - 1)) ^ L::flip(r);
+        const bool in = row0 + r < rows && c * EPC < channels;
+        const T* src = base + (size_t)(row0 + r) * ld + c * EPC;
+        copy_to_lds(in ? (const void*)src : (const void*)&g_zero_row, lds + j * L::PITCH);
+    }
+}
+
+// Fragment kf of the 32 rows that start at `row` (a multiple of 32).
+template <typename T, int CP>
+__device__ inline u32x4 row_fragment(const char* lds, int row, int kf, int lane) {
+    typedef Tile<T, CP> L;
+    const int r = lane & 31, low = ((2 * kf) & L::MASK) + (lane >> 5);
+    return *(const u32x4*)(lds + L::row(row) + (((2 * kf) & ~L::MASK) << 4) + L::row(r) + ((low ^ L::flip(r)) << 4));
+}
+
+// Fragment of owner rows straight from memory.
+template <typename T, int CP>
+__device__ inline void own_fragments(u32x4 (&q)[CP / Wide<T>::KF], const BankArgs& a, int own0, int lane, bool negate) {
+    constexpr int EPC = 16 / (int)sizeof(T);
+    const uint32_t flip = !negate ? 0u : sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    const int row = own0 + (lane & 31);
+#pragma unroll
+    for (int kf = 0; kf < CP / Wide<T>::KF; ++kf) {
+        const int c = (kf * 2 + (lane >> 5)) * EPC;
+        q[kf] = row < a.n_own && c < a.channels ? *(const u32x4*)((const T*)a.own + (size_t)row * a.ld_own + c) : u32x4{0, 0, 0, 0};
+        q[kf] ^= flip;
+    }
+}
+
+// The compiler would read all fragments ahead and run out of registers: it may not look further ahead than `AHEAD` of them.
+template <typename T, int CP>
+__device__ inline f32x16_t products(const char* lds, int row, const u32x4 (&q)[CP / Wide<T>::KF], int lane) {
+    constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;
+    f32x16_t acc = {};
+#pragma unroll
+    for (int kf = 0; kf < CP / Wide<T>::KF; ++kf) {
+        Wide<T>::run(acc, row_fragment<T, CP>(lds, row, kf, lane), q[kf]);
+        if (kf % AHEAD == AHEAD - 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    return acc;
+}
+
+struct __attribute__((packed, aligned(4))) LooseQuad { f32x4 v; };
+
+// Weights of the lane's 16 other rows j0 + 8 b + 4 g + i, 0 beyond `end`; w: the row of weights of the lane's feature row.
+__device__ inline void row_weights(float wv[16], const float* w, int j0, int g, int end) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int j = j0 + 8 * b + 4 * g;
+        if (j0 + 32 <= end) {
+            const f32x4 q = ((const LooseQuad*)(w + j))->v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wv[4 * b + i] = q[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wv[4 * b + i] = j + i < end ? w[j + i] : 0.0f;
+        }
+    }
+}
+
+
+void launch_bank_gradient(const BankArgs& a, int dtype, bool own_bank, hipStream_t st);
+void launch_bank_coef(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse, const long long* targets, int rows,
+                      int cols, float* coef, bool join_m, hipStream_t st);
+
+// The six arrays that the gradient kernels need of every feature row; rows beyond the last have p = 0 and no target.
+enum { K_M, K_LOG2_S, K_C, K_G2, K_LOGP, K_TARGET, K_COUNT };
+constexpr int coef_rows(int64_t rows) { return (int)((rows + 63) / 64 * 64 + 64); }
+
+inline int padded_channels(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : 256; }
+
+}  // namespace nemo

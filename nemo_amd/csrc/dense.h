@@ -65,6 +65,11 @@ __device__ inline void copy_to_lds(const void* g, void* lds) {
     __builtin_amdgcn_global_load_lds((NEMO_GLOBAL void*)g, (NEMO_LDS void*)lds, 16, 0, 0);
 }
 
+// The same with 4 bytes a lane, 256 bytes of LDS.
+__device__ inline void copy_words_to_lds(const void* g, void* lds) {
+    __builtin_amdgcn_global_load_lds((NEMO_GLOBAL void*)g, (NEMO_LDS void*)lds, 4, 0, 0);
+}
+
 // ---- reductions -----------------------------------------------------------------------------------------------------------------
 __device__ inline float wave_sum(float v) {
 #pragma unroll

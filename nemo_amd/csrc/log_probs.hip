@@ -68,15 +68,12 @@ __device__ inline void add_scores(SoftmaxState& a, const float z[N]) {
     float m = a.m;
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
-    const float d = a.m - m, f = fast_exp(d);
-    a.t = f * (a.t + fmaxf(d, -200.0f) * a.s);
-    a.s *= f;
-    a.m = m;
+    raise(a, m, kLog2e);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float dz = z[i] - m, e = fast_exp(dz);
+        const float x = (z[i] - m) * kLog2e, e = exp2_fast(x);
         a.s += e;
-        a.t += weighted(e, dz);
+        a.t += e * fmaxf(x, -200.0f);                                  // 0 where e is 0, also where x is -inf
     }
 }
 
@@ -108,7 +105,7 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
             }
         }
     }
-    st = wave_join(st);
+    st = wave_join(st, kLog2e);
     __shared__ SoftmaxState s_state[4];
     __shared__ Entry s_top[TOP ? 4 : 1][kMaxTop];
     const int top = a.out.top;
@@ -143,7 +140,7 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
         if (wr != 0 || !live) return;
         st = s_state[wave];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) st = join_states(st, s_state[wave + i]);
+        for (int i = 1; i < WAVES; ++i) st = join_states(st, s_state[wave + i], kLog2e);
     } else {
         if (TOP) __syncthreads();
         if (!live) return;
@@ -190,7 +187,7 @@ __global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a) {
     const size_t at = (size_t)lane * a.rows + row, plane = (size_t)a.parts * a.rows;
     SoftmaxState st = empty_state();
     if (lane < a.parts) st = {a.part_state[at], a.part_state[plane + at], a.part_state[2 * plane + at]};
-    st = wave_join(st);
+    st = wave_join(st, kLog2e);
     if (lane == 0) {
         const long long t = a.targets[row];
         float zt = 0.0f;
@@ -226,7 +223,12 @@ __global__ __launch_bounds__(256) void log_probs_backward_kernel(LogProbArgs a, 
             chunk_scores<T>(logits, w, a.scale, j, a.cols, z);
             union { u32x4 u; T t[N]; } c;
 #pragma unroll
-            for (int i = 0; i < N; ++i) c.t[i] = from_f32<T>(a.scale * score_gradient(k, z[i], j + i));
+            for (int i = 0; i < N; ++i) {
+                float d = prob_gradient(__builtin_fmaf(z[i] - k.m, kLog2e, -k.log2_s), k.c, k.g2);
+                if (j + i == k.target) d += k.g_logp;
+                if (z[i] == neg_inf()) d = 0.0f;
+                c.t[i] = from_f32<T>(a.scale * d);
+            }
             if (j + N <= a.cols) {
                 ((LooseChunk<T>*)(out + j))->v = c.u;
             } else {
@@ -306,7 +308,7 @@ extern "C" int nemo_log_probs(const void* logits, int64_t ld, const float* weigh
         a.part_z = (float*)ws;
         a.part_place = (int*)(ws + align256((size_t)a.parts * rows * top * 4));
     }
-    a.out = {out_logp, out_entropy, out_lse, out_stats, out_top_logp, (long long*)out_top_index, top};
+    a.out = {out_logp, out_entropy, out_lse, out_stats, out_top_logp, (long long*)out_top_index, top, 0.0f};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == NEMO_F32) launch_log_probs<float>(a, st);
     else if (dtype == NEMO_BF16) launch_log_probs<bf16>(a, st);
