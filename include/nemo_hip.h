@@ -474,7 +474,7 @@ int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights
 /* nemo_log_probs straight from features [rows,channels] and bank [cols,channels] (f32 or bf16, both the same):
  *   z[i,j] = scale <features[i], bank[j]> - weights[i,j],
  * same outputs and rules, the [rows,cols] matrix is never written.  Products are summed in f32 (f32: on the f32 matrix cores).  channels
- * 1..256 (padded to 32, 64, 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same
+ * 1..256 (padded to 64, 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same
  * pointers and strides (rows that do not start on 16 bytes are copied into it), contents undefined before and after. */
 size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                      int64_t channels, int32_t dtype, int32_t top);

@@ -1,0 +1,235 @@
+// The log probabilities of log_probs.hip straight from features and bank, z = scale <feature, bank row> - weight, without ever writing the
+// [rows, bank rows] matrix: owners (bank_tiles.h) are the feature rows, others the bank; the softmax state of a row and its best entries live
+// in the lane, no exchange until the end.  The bank is split where there are too few feature rows to fill the device; states and lists of the
+// parts, and of the two lanes of a row, are joined by a second kernel in a fixed order.  Compiled once for each element type (NEMO_ELEMENT).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/nemo_hip.h"
+#include "bank_tiles.h"
+
+namespace nemo {
+
+// Puts v into the list, ordered by v * order (the score; a score is not smaller where the product is not, but may be equal).  Places arrive
+// in rising order, so an equal score goes behind those already there.
+template <int TOP>
+__device__ inline void insert(float (&tv)[TOP], int (&tp)[TOP], float v, int place, float order) {
+    const float z = v * order;
+#pragma unroll
+    for (int i = TOP - 1; i >= 0; --i) {
+        const bool above = z > tv[i] * order;
+        const bool shift = i > 0 && z > tv[i > 0 ? i - 1 : 0] * order;
+        if (above) {
+            tv[i] = shift ? tv[i > 0 ? i - 1 : 0] : v;
+            tp[i] = shift ? tp[i > 0 ? i - 1 : 0] : place;
+        }
+    }
+}
+
+// GENERAL: with weights, or with hardly any scale; see softmax_state.h for the two forms of the state.  The sign of the scale goes into the
+// owners' fragments where the state is kept of the products.
+//
+// Tiles of 32 bank rows; in step n the wave multiplies tile n + 1 while it takes the products of tile n into the state, so that matrix cores
+// and vector units work side by side.  Two tiles in LDS (n + 1, and n + 2 on its way), one barrier a step.
+template <typename T, int CP, int TOP, bool GENERAL>
+__global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forward_kernel(BankArgs a) {
+    typedef Tile<T, CP> L;
+    constexpr int NT = TOP > 0 ? TOP : 1, NKF = CP / Wide<T>::KF;
+    constexpr bool F32 = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(16))) char lds0[L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[L::BYTES];
+    __shared__ int s_again;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const int part = (int)(blockIdx.x % a.parts);
+    const int own0 = (int)(blockIdx.x / a.parts) * 128 + wave * 32, row = own0 + (lane & 31);
+    const bool live = row < a.n_own;
+    u32x4 q[NKF];
+    own_fragments<T, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
+    const float* w = a.weights ? a.weights + (live ? row : 0) * a.ldw : nullptr;
+    const long long tl = live ? a.targets[row] : -1;
+    const int target = tl >= 0 && tl < a.n_other ? (int)tl : -1;
+    const float scale = GENERAL ? a.scale : __builtin_fabsf(a.scale);
+    const float k = a.out.k, order = GENERAL ? 1.0f : scale, unit = GENERAL ? kLog2e : 1.0f;
+    SoftmaxState st;
+    float tv[NT];
+    int tp[NT];
+
+    auto load_weights = [&](float (&wv)[16], int tile) __attribute__((always_inline)) {
+        if (GENERAL && w) row_weights(wv, w, tile * 32, g, a.n_other);
+    };
+    // a product, or the score if GENERAL
+    auto value = [&](const f32x16_t& pr, const float (&wv)[16], int i) __attribute__((always_inline)) {
+        return !GENERAL ? pr[i] : w ? score(pr[i], scale, wv[i]) : score(pr[i], scale);
+    };
+    auto peak_of = [&](const float (&v)[16]) __attribute__((always_inline)) {
+        float peak = v[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) peak = fmaxf(peak, v[i]);
+        return peak;
+    };
+    // adds a value to the state.  SAFE: also right where a difference of two products is beyond the range of f32
+    auto add = [&](float v, auto safe_tag) __attribute__((always_inline)) {
+        constexpr bool SAFE = decltype(safe_tag)::value || GENERAL;
+        const float x = GENERAL ? (v - st.m) * kLog2e : __builtin_fmaf(k, v, -st.m), e = exp2_fast(x);
+        st.s += e;
+        st.t += e * (SAFE ? fmaxf(x, -200.0f) : x);                    // 0 where e is 0, also where x is -inf
+    };
+    // what only some tiles have: the target's score, entries for the list
+    auto note = [&](const float (&v)[16], int tile) __attribute__((always_inline)) {
+        const int j0 = tile * 32;
+        if (__any(target >= j0 && target < j0 + 32)) {
+            const int at = target - j0 - 4 * g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (at == 8 * (i >> 2) + (i & 3)) a.z_target[row] = v[i];
+        }
+        if (TOP > 0) {
+            float peak = v[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) peak = fmaxf(peak, v[i]);
+            if (__any(peak * order > tv[NT - 1] * order)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (__any(v[i] * order > tv[NT - 1] * order)) insert(tv, tp, v[i], j0 + 8 * (i >> 2) + 4 * g + (i & 3), order);
+            }
+        }
+    };
+    const int tiles = (a.n_other + 31) / 32;
+    const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
+    const Stager<T, CP> stager((const T*)a.other, a.ld_other, a.n_other, a.channels, wave, lane);
+    auto stage = [&](char* lds, int tile) __attribute__((always_inline)) { stager.copy(lds, tile); };
+    auto start = [&]() __attribute__((always_inline)) {
+        st = empty_state();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) { tv[i] = neg_inf(); tp[i] = kNoPlace; }
+    };
+    // tiles from `t` on one step after the other, with every precaution
+    auto plain_pass = [&](int t) __attribute__((always_inline)) {
+        for (; t < t1; ++t) {
+            __syncthreads();
+            stage(lds0, t);
+            float wv[16], v[16];
+            load_weights(wv, t);
+            __syncthreads();
+            const f32x16_t pr = products<T, CP>(lds0, q, lane);
+            const int left = a.n_other - t * 32 - 4 * g;               // registers whose row 8 b + i is at least this are beyond the end
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 8 * (i >> 2) + (i & 3) >= left ? neg_inf() : value(pr, wv, i);
+            const float peak = peak_of(v);
+            raise(st, fmaxf(st.m, GENERAL ? peak : k * peak), unit);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) add(v[i], std::true_type{});
+            note(v, t);
+        }
+    };
+    start();
+    // the last tile of the bank may be cut short: it is left to the plain pass
+    const int whole = t1 == tiles && a.n_other % 32 != 0 && t1 > t0 ? t1 - 1 : t1;
+    if (t0 < whole) {
+        stage(lds0, t0);
+        __syncthreads();
+        f32x16_t pr = products<T, CP>(lds0, q, lane);
+        stage(lds1, t0 + 1);
+        // `next` holds tile t + 1; `after` held tile t, whose products are in pr.  A slice: a fragment is read (two slices ahead of its use),
+        // multiplied, and a share of the 18 units of tile t is done: the largest product, the state raised to it, 16 products added.  Weights
+        // may arrive during the first half of the slices.
+        auto step = [&](int t, const char* next, char* after) __attribute__((always_inline)) {
+            __syncthreads();                                           // tile t + 1 is there; nobody reads tile t any more
+            stage(after, t + 2);                                       // also behind the part's last tile, to no effect: no branch
+            float wv[16], v[16];
+            load_weights(wv, t);
+            f32x16_t nxt = {};
+            constexpr int UNITS = 18;
+            float peak = 0.0f;
+            u32x4 f[3];
+            f[0] = row_fragment<T, CP>(next, 0, lane);
+            f[1] = row_fragment<T, CP>(next, 1, lane);
+#pragma unroll
+            for (int i = 0; i < NKF; ++i) {
+                if (i + 2 < NKF) f[(i + 2) % 3] = row_fragment<T, CP>(next, i + 2, lane);
+                settle(f[i % 3]);
+                Wide<T>::run(nxt, f[i % 3], q[i]);
+                const int from = GENERAL ? (2 * i < NKF ? 0 : (2 * i - NKF) * UNITS / NKF) : i * UNITS / NKF;
+                const int to = GENERAL ? (2 * i + 2 < NKF ? 0 : (2 * i + 2 - NKF) * UNITS / NKF) : (i + 1) * UNITS / NKF;
+#pragma unroll
+                for (int u = from; u < to; ++u) {
+                    if (u == 0) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = value(pr, wv, e);
+                        peak = peak_of(v);
+                        settle(peak);
+                    }
+                    if (u == 1) {
+                        raise(st, fmaxf(st.m, GENERAL ? peak : k * peak), unit);
+                        settle(st.m);
+                        settle(st.s);
+                    }
+                    if (u >= 2) {
+                        add(v[u - 2], std::false_type{});
+                        settle(st.s);
+                        settle(st.t);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            note(v, t);
+            pr = nxt;
+        };
+        int t = t0;                                                    // no way out of the loop's middle: it would cost copies of registers
+        for (; t + 2 <= whole; t += 2) {
+            step(t, lds1, lds0);
+            step(t + 1, lds0, lds1);
+        }
+        if (t < whole) step(t, lds1, lds0);
+    }
+    plain_pass(whole);
+    if (!GENERAL) {
+        // a difference beyond the range, times the 0 that its exponential is, would have spoilt t alone
+        if (threadIdx.x == 0) s_again = 0;
+        __syncthreads();
+        if (st.t != st.t && st.s == st.s) s_again = 1;
+        __syncthreads();
+        if (s_again) {
+            start();
+            plain_pass(t0);
+        }
+    }
+    if (!live) return;
+    const size_t rows = a.n_own, at = (size_t)(part * 2 + g) * rows + row, plane = (size_t)2 * a.parts * rows;
+    a.part_state[at] = st.m;
+    a.part_state[plane + at] = st.s;
+    a.part_state[2 * plane + at] = st.t;
+#pragma unroll
+    for (int i = 0; i < TOP; ++i)
+        if (i < a.out.top) {
+            a.part_z[at * a.out.top + i] = tv[i];
+            a.part_place[at * a.out.top + i] = tp[i];
+        }
+}
+
+template <typename T, int CP>
+static void launch(const BankArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)((a.n_own + 127) / 128 * a.parts));
+    const int top = a.out.top;
+    const bool general = a.out.k == 0.0f;
+    if (top == 0) {
+        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, false>), grid, dim3(256), 0, st, a);
+    } else if (top <= 5) {
+        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, false>), grid, dim3(256), 0, st, a);
+    } else {
+        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, false>), grid, dim3(256), 0, st, a);
+    }
+}
+
+template <> void launch_bank_forward<NEMO_ELEMENT>(const BankArgs& a, hipStream_t st) {
+    switch (padded_channels(a.channels)) {
+        case 64: launch<NEMO_ELEMENT, 64>(a, st); break;
+        case 128: launch<NEMO_ELEMENT, 128>(a, st); break;
+        default: launch<NEMO_ELEMENT, 256>(a, st);
+    }
+}
+
+}  // namespace nemo

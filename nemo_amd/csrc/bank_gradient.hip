@@ -6,7 +6,8 @@
 //     bank's gradient      owners = bank rows, others = features; what dz needs of a feature row is staged beside the tile
 // In bf16 dz is split into two pieces, dz = hi + lo, each of them multiplied: a single piece would put an error of 2^-9 of the largest term into
 // sums whose terms largely cancel (the target's against all others').  The other axis is split where there are too few owners to fill the
-// device; the parts are joined in their order by a second kernel.  Results of two calls are the same bits.
+// device; the parts are joined in their order by a second kernel.  Results of two calls are the same bits.  Compiled once for each element type
+// (NEMO_ELEMENT).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -14,20 +15,6 @@
 #include "bank_tiles.h"
 
 namespace nemo {
-
-__global__ __launch_bounds__(256) void bank_coef_kernel(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse,
-                                                        const long long* targets, int rows, int cols, float* coef, bool join_m) {
-    const int row = blockIdx.x * 256 + threadIdx.x, n = coef_rows(rows);
-    if (row >= n) return;
-    RowCoef k = {0.0f, __builtin_inff(), 0.0f, 0.0f, 0.0f, -1};
-    if (row < rows) k = row_coef(stats, g_logp, g_entropy, g_lse, targets, row, cols);
-    coef[K_M * n + row] = join_m ? k.m + k.log2_s : k.m;
-    coef[K_LOG2_S * n + row] = k.log2_s;
-    coef[K_C * n + row] = k.c;
-    coef[K_G2 * n + row] = k.g2;
-    coef[K_LOGP * n + row] = k.g_logp;
-    coef[K_TARGET * n + row] = __builtin_bit_cast(float, k.target);
-}
 
 // dz of one score or product without the target's share.  In bf16 and without weights m holds m + log2 s, one operation less: off by u |lse|
 // (1e-6 at 16), far below the rounding of dz's pieces.  SAFE: log2 p may be -inf.
@@ -48,27 +35,25 @@ __device__ inline float clean_value(float v) { return __builtin_fabsf(v) <= FLT_
 // 16 b + 8 (e / 4) + 4 g + e % 4, two transposing reads of four rows each (lane i of a group of 16 supplies columns 4 (i % 4) .. + 3 of row
 // i / 4 and receives column i of the four rows).
 template <typename T, int CP>
-__device__ inline u32x4 column_fragment(const char* lds, int row0, int b, int cb, int lane, bool clean) {
+__device__ inline u32x4 column_fragment(const char* lds, int b, int cb, int lane, bool clean) {
     typedef Tile<T, CP> L;
     const int g = lane >> 5;
     if constexpr (sizeof(T) == 4) {
         u32x4 v;
-        const int low = (lane & 31) >> 2;                              // chunk within the 32 columns; flip reaches no further
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int f = L::RPI == 8 ? 4 * g + i : L::flip(i);        // flip of row 8 b + 4 g + i
-            float x = *(const float*)(lds + L::row(row0) + L::row(8 * b + i) + cb * 4 + L::row(4) * g + ((low ^ f) << 4) + (lane & 3) * 4);
+            float x = *(const float*)(lds + L::row(8 * b + i) + L::row(4) * g + L::chunk(cb >> 2, (lane & 31) >> 2, L::flip(4 * g + i)) + (lane & 3) * 4);
             if (clean) x = clean_value(x);
             v[i] = __builtin_bit_cast(uint32_t, x);
         }
         return v;
     } else {
-        const int i = lane & 15, t = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), r = 4 * g + (i >> 2);
-        const int low = (((cb >> 3) & L::MASK) + t) ^ L::flip(r);
-        const char* at = lds + L::row(row0) + L::row(16 * b) + (((cb >> 3) & ~L::MASK) << 4) + L::row(4) * g + L::row(i >> 2) + (low << 4) + (i & 1) * 8;
+        const int i = lane & 15, t = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
         union { i16x4 h[2]; u32x4 v; bf16 t[8]; } u;
-        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NEMO_LDS i16x4*)at);
-        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NEMO_LDS i16x4*)(at + (L::RPI >= 16 ? 8 * L::RB : L::row(8))));
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            u.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (NEMO_LDS i16x4*)(lds + L::row(16 * b + 8 * e) + L::row(4) * g + L::row(i >> 2) + L::chunk(cb >> 3, t, L::flip(8 * e + 4 * g + (i >> 2))) + (i & 1) * 8));
         if (clean)
 #pragma unroll
             for (int e = 0; e < 8; ++e) u.t[e] = (bf16)clean_value((float)u.t[e]);
@@ -76,178 +61,302 @@ __device__ inline u32x4 column_fragment(const char* lds, int row0, int b, int cb
     }
 }
 
-// OWN_BANK: owners are bank rows, others features.  The products of places that are left out must not count even where a feature or bank row
-// holds infinities or NaN (0 x NaN): when a wave ends with a value that is not finite, its workgroup goes through its part again with such
-// values of the second product's first operand taken as 0 (and with log2 p = -inf allowed for).  Where they are not left out the scores themselves, and with them dz, are NaN, and
+// 16 dz of a lane as second operands of the second product: f32 as they are; bf16 as two pieces each, filled two values at a time.
+template <typename T> struct Pieces;
+template <> struct Pieces<float> {
+    static constexpr int STEPS = 4, N = 1;
+    u32x4 p[4][1];
+    __device__ inline void pair(int i, float z0, float z1) {
+        p[i >> 1][0][2 * (i & 1)] = __builtin_bit_cast(uint32_t, z0);
+        p[i >> 1][0][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, z1);
+    }
+    __device__ inline void settle_pair(int) {}
+};
+template <> struct Pieces<bf16> {
+    static constexpr int STEPS = 2, N = 2;
+    u32x4 p[2][2];
+    __device__ inline void pair(int i, float z0, float z1) {
+        typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 hi = {(bf16)z0, (bf16)z1};
+        const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+        const float h0 = __builtin_bit_cast(float, h << 16), h1 = __builtin_bit_cast(float, h & 0xFFFF0000u);
+        const bf16x2 lo = {(bf16)(z0 - h0), (bf16)(z1 - h1)};
+        p[i >> 2][0][i & 3] = h;
+        p[i >> 2][1][i & 3] = __builtin_bit_cast(uint32_t, lo);
+    }
+    __device__ inline void settle_pair(int i) {
+        uint32_t h = p[i >> 2][0][i & 3], l = p[i >> 2][1][i & 3];
+        asm volatile("" : "+v"(h), "+v"(l));
+        p[i >> 2][0][i & 3] = h;
+        p[i >> 2][1][i & 3] = l;
+    }
+};
+
+template <typename T, int CP>
+__device__ inline void second_product(f32x16_t (&acc)[CP / 32], const char* lds, const Pieces<T>& dz, int lane, bool clean) {
+#pragma unroll
+    for (int b = 0; b < Pieces<T>::STEPS; ++b)
+#pragma unroll
+        for (int x = 0; x < CP / 32; ++x) {
+            const u32x4 f = column_fragment<T, CP>(lds, b, x * 32, lane, clean);
+#pragma unroll
+            for (int n = 0; n < Pieces<T>::N; ++n) Wide<T>::run(acc[x], f, dz.p[b][n]);
+        }
+}
+
+// OWN_BANK: owners are bank rows, others features.  GENERAL as in the forward kernel.
+//
+// Tiles of 32 other rows.  Matrix cores and vector units work side by side only if a wave has something for both: in step n it multiplies
+// tile n + 1 (first product), computes dz of tile n from the products of the step before, and multiplies the dz of tile n - 1 (second product),
+// none of which waits for another; the instructions are interleaved in slices that the compiler may not mix.  That takes four tiles in LDS (n - 1, n,
+// n + 1 and n + 2 on its way), one barrier a step, and straight code: the targets' share of dz is left out of it.  In the features' gradient it
+// is one bank row a feature row, added at the end; in the bank's gradient a step in which some feature row's target is among the owners adds
+// it by a second product of its own.  At 256 channels there are not enough registers for two steps at once: one after the other.
+//
+// Products of places that are left out must not count even where a feature or bank row holds infinities or NaN (0 x NaN): when a wave ends with
+// a value that is not finite, its workgroup goes through its part again, step after step, with such values of the second product's first
+// operand taken as 0 and with log2 p = -inf allowed for.  Where they are not left out the scores themselves, and with them dz, are NaN, and
 // so stays the result.
-// GENERAL as in the forward kernel.
 template <typename T, int CP, bool OWN_BANK, bool GENERAL>
 __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(BankArgs a) {
-    constexpr int BJ = Tile<T, CP>::ROWS;
+    typedef Tile<T, CP> L;
     constexpr bool F32 = sizeof(T) == 4, SPLIT = GENERAL || F32;       // log2 s apart from m
-    __shared__ __attribute__((aligned(16))) char lds0[Tile<T, CP>::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds1[Tile<T, CP>::BYTES];
+    constexpr int NX = CP / 32, NKF = CP / Wide<T>::KF;
+    __shared__ __attribute__((aligned(16))) char lds0[L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds2[L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds3[L::BYTES];
     __shared__ __attribute__((aligned(16))) float s_coef0[OWN_BANK ? K_COUNT : 1][64];
     __shared__ __attribute__((aligned(16))) float s_coef1[OWN_BANK ? K_COUNT : 1][64];
+    __shared__ __attribute__((aligned(16))) float s_coef2[OWN_BANK ? K_COUNT : 1][64];
+    __shared__ __attribute__((aligned(16))) float s_coef3[OWN_BANK ? K_COUNT : 1][64];
     __shared__ int s_again;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int part = (int)(blockIdx.x % a.parts);
     const int own0 = (int)(blockIdx.x / a.parts) * 128 + wave * 32, own = own0 + (lane & 31);
     const bool live = own < a.n_own;
-    u32x4 q[CP / Wide<T>::KF];
+    u32x4 q[NKF];
     own_fragments<T, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
     const int n_coef = coef_rows(OWN_BANK ? a.n_other : a.n_own);
     const float k = a.out.k;
-    float m = 0.0f, log2_s = __builtin_inff(), c = 0.0f, g2 = 0.0f, gl = 0.0f;     // of an owner beyond the last
-    int target = -1;
+    float m = 0.0f, log2_s = 0.0f, c = 0.0f, g2 = 0.0f;               // of an owner beyond the last: dz = 0
     const float* w = nullptr;
     if (!OWN_BANK && live) {
         m = a.coef[K_M * n_coef + own];
         log2_s = a.coef[K_LOG2_S * n_coef + own];
         c = a.coef[K_C * n_coef + own];
         g2 = a.coef[K_G2 * n_coef + own];
-        gl = a.coef[K_LOGP * n_coef + own];
-        target = __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + own]);
     }
     if (GENERAL && a.weights) w = OWN_BANK ? a.weights + (live ? own : 0) : a.weights + (live ? own : 0) * a.ldw;
-    f32x16_t acc[CP / 32];
+    f32x16_t acc[NX];
 
+    const Stager<T, CP> stager((const T*)a.other, a.ld_other, a.n_other, a.channels, wave, lane);
     auto stage = [&](char* lds, float (*coef)[64], int tile) __attribute__((always_inline)) {
-        stage_rows<T, CP>(lds, (const T*)a.other, a.ld_other, tile * BJ, a.n_other, a.channels, wave, lane);
+        stager.copy(lds, tile);
         if (OWN_BANK) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (wave + 4 * i < K_COUNT)
-                    copy_words_to_lds(a.coef + (size_t)(wave + 4 * i) * n_coef + tile * BJ + lane, &coef[OWN_BANK ? wave + 4 * i : 0][0]);
+                    copy_words_to_lds(a.coef + (size_t)(wave + 4 * i) * n_coef + tile * 32 + lane, &coef[OWN_BANK ? wave + 4 * i : 0][0]);
         }
     };
-    auto consume = [&](const char* lds, const float (*coef)[64], int tile, auto clean_tag) __attribute__((always_inline)) {
-        constexpr bool CLEAN = decltype(clean_tag)::value, SAFE = GENERAL || CLEAN;
-#pragma unroll 1
-        for (int s = 0; s < BJ / 32; ++s) {
-            const int j0 = tile * BJ + s * 32;
-            float wv[16];
-            if (GENERAL && w) {
-                if (!OWN_BANK) {
-                    row_weights(wv, w, j0, g, a.n_other);
-                } else {
+    auto load_weights = [&](float (&wv)[16], int tile) __attribute__((always_inline)) {
+        if (!GENERAL || !w) return;
+        const int j0 = tile * 32;
+        if (!OWN_BANK) {
+            row_weights(wv, w, j0, g, a.n_other);
+        } else if (j0 + 32 <= a.n_other) {
+            // 32-bit offsets of a lane from addresses that all lanes share
+            const uint32_t at = (uint32_t)((live ? own : 0) + 4 * g * (int)a.ldw);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        wv[i] = w[(size_t)min(j0 + 8 * (i >> 2) + 4 * g + (i & 3), a.n_other - 1) * a.ldw];
-                }
+            for (int i = 0; i < 16; ++i) wv[i] = (a.weights + (size_t)(j0 + 8 * (i >> 2) + (i & 3)) * a.ldw)[at];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = j0 + 8 * (i >> 2) + 4 * g + (i & 3);
+                wv[i] = j < a.n_other ? w[(size_t)j * a.ldw] : __builtin_inff();
             }
-            const f32x16_t pr = products<T, CP>(lds, s * 32, q, lane);
-            float z[16];
+        }
+    };
+    // what dz needs of the four feature rows 8 b + 4 g + i, or of the owner
+    struct Quad { f32x4 m, s, c, g2; };
+    auto quad = [&](const float (*coef)[64], int b) __attribute__((always_inline)) {
+        Quad k4 = {{m, m, m, m}, {log2_s, log2_s, log2_s, log2_s}, {c, c, c, c}, {g2, g2, g2, g2}};
+        if (OWN_BANK) {
+            const int r = 8 * b + 4 * g;
+            k4.m = *(const f32x4*)&coef[K_M][r];
+            k4.c = *(const f32x4*)&coef[OWN_BANK ? K_C : 0][r];
+            k4.g2 = *(const f32x4*)&coef[OWN_BANK ? K_G2 : 0][r];
+            if (SPLIT) k4.s = *(const f32x4*)&coef[OWN_BANK ? K_LOG2_S : 0][r];
+        }
+        return k4;
+    };
+    // product i of a tile -> dz without the targets' share
+    auto differentiate = [&](const f32x16_t& pr, const float (&wv)[16], const Quad& k4, int i, int tile, auto safe_tag) __attribute__((always_inline)) {
+        constexpr bool SAFE = decltype(safe_tag)::value || GENERAL;
+        const float s = !GENERAL ? pr[i] : w ? score(pr[i], a.scale, wv[i]) : score(pr[i], a.scale);
+        const float d = pair_gradient<T, GENERAL, SAFE>(s, k, k4.m[i & 3], k4.s[i & 3], k4.c[i & 3], k4.g2[i & 3]);
+        // rows beyond the last are zeros, but where all scores are far below 0 the probability of a 0 is not even finite
+        return SAFE && !GENERAL && !OWN_BANK && tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= a.n_other ? 0.0f : d;
+    };
+    // the targets' share in the bank's gradient: feature rows of this tile whose target is an owner
+    auto add_targets = [&](const char* lds, const float (*coef)[64], int tile, bool clean) __attribute__((always_inline)) {
+        if (!OWN_BANK) return;
+        const int t = __builtin_bit_cast(int, coef[OWN_BANK ? K_TARGET : 0][lane & 31]);
+        if (!__any(t >= own0 && t < own0 + 32)) return;
+        float z[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = !GENERAL ? pr[i] : w ? score(pr[i], a.scale, wv[i]) : score(pr[i], a.scale);
-            // dz; the target's share only where the block holds some target
-            if (!OWN_BANK) {
-                const bool hit = __any(target >= j0 && target < j0 + 32);
-                const int at = target - j0 - 4 * g, left = a.n_other - j0 - 4 * g;
-                uint32_t gone = 0;
-                if (GENERAL && hit) {
+        for (int i = 0; i < 16; ++i) {
+            const int r = 8 * (i >> 2) + 4 * g + (i & 3);
+            const int tr = __builtin_bit_cast(int, coef[OWN_BANK ? K_TARGET : 0][r]);
+            z[i] = tr == own ? coef[OWN_BANK ? K_LOGP : 0][r] : 0.0f;
+            // an owner that is left out for that row
+            if (GENERAL && w && tr == own && w[(size_t)(tile * 32 + r) * a.ldw] == __builtin_inff()) z[i] = 0.0f;
+        }
+        Pieces<T> dz;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) gone |= z[i] == neg_inf() ? 1u << i : 0u;
-                }
+        for (int i = 0; i < 8; ++i) dz.pair(i, z[2 * i], z[2 * i + 1]);
+        second_product<T, CP>(acc, lds, dz, lane, clean);
+    };
+    const int tiles = (a.n_other + 31) / 32;
+    const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
+
+    // one step after the other
+    auto plain_pass = [&](auto clean_tag) __attribute__((always_inline)) {
+        constexpr bool CLEAN = decltype(clean_tag)::value;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] = pair_gradient<T, GENERAL, SAFE>(z[i], k, m, log2_s, c, g2);
-                if (hit) {
+        for (int x = 0; x < NX; ++x) acc[x] = {};
+        auto one = [&](const char* lds, const float (*coef)[64], int tile) __attribute__((always_inline)) {
+            float wv[16];
+            load_weights(wv, tile);
+            const f32x16_t pr = products<T, CP>(lds, q, lane);
+            Pieces<T> dz;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (at == 8 * (i >> 2) + (i & 3) && !(gone >> i & 1)) z[i] += gl;
-                }
-                if (j0 + 32 > a.n_other) {
+            for (int b = 0; b < 4; ++b) {
+                const Quad k4 = quad(coef, b);
+                float z[4];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (8 * (i >> 2) + (i & 3) >= left) z[i] = 0.0f;
-                }
-            } else {
-                const int t = __builtin_bit_cast(int, coef[K_TARGET][s * 32 + (lane & 31)]);
-                const bool hit = __any(t >= own0 && t < own0 + 32);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int r = s * 32 + 8 * b + 4 * g;
-                    const f32x4 km = *(const f32x4*)&coef[K_M][r], kc = *(const f32x4*)&coef[K_C][r], kg = *(const f32x4*)&coef[K_G2][r];
-                    f32x4 ks = {};
-                    if (SPLIT) ks = *(const f32x4*)&coef[K_LOG2_S][r];
-                    if (!hit) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            z[4 * b + i] = pair_gradient<T, GENERAL, SAFE>(z[4 * b + i], k, km[i], ks[i], kc[i], kg[i]);
-                    } else {
-                        const f32x4 kl = *(const f32x4*)&coef[K_LOGP][r], kt = *(const f32x4*)&coef[K_TARGET][r];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float v = z[4 * b + i], d = pair_gradient<T, GENERAL, SAFE>(v, k, km[i], ks[i], kc[i], kg[i]), tb = kt[i];
-                            z[4 * b + i] = __builtin_bit_cast(int, tb) == own && !(GENERAL && v == neg_inf()) ? d + kl[i] : d;
-                        }
-                    }
-                }
+                for (int i = 0; i < 4; ++i) z[i] = differentiate(pr, wv, k4, 4 * b + i, tile, clean_tag);
+                dz.pair(2 * b, z[0], z[1]);
+                dz.pair(2 * b + 1, z[2], z[3]);
             }
             __builtin_amdgcn_sched_barrier(0);
-            // the second product; fragments are read one step ahead of the matrix cores, no further
-            if constexpr (F32) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const f32x4 d = {z[4 * b], z[4 * b + 1], z[4 * b + 2], z[4 * b + 3]};
-                    const u32x4 dq = __builtin_bit_cast(u32x4, d);
-#pragma unroll
-                    for (int x = 0; x < CP / 32; ++x) {
-                        Wide<T>::run(acc[x], column_fragment<T, CP>(lds, s * 32, b, x * 32, lane, CLEAN), dq);
-                        if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    bf16x8 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        hi[e] = (bf16)z[8 * b + e];
-                        lo[e] = (bf16)(z[8 * b + e] - (float)hi[e]);
-                    }
-                    const u32x4 hq = __builtin_bit_cast(u32x4, hi), lq = __builtin_bit_cast(u32x4, lo);
-#pragma unroll
-                    for (int x = 0; x < CP / 32; ++x) {
-                        const u32x4 p = column_fragment<T, CP>(lds, s * 32, b, x * 32, lane, CLEAN);
-                        Wide<T>::run(acc[x], p, hq);
-                        Wide<T>::run(acc[x], p, lq);
-                        if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            }
-        }
-    };
-    const int tiles = (a.n_other + BJ - 1) / BJ;
-    const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
-    auto pass = [&](auto clean_tag) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < CP / 32; ++x) acc[x] = {};
+            second_product<T, CP>(acc, lds, dz, lane, CLEAN);
+            add_targets(lds, coef, tile, CLEAN);
+        };
         if (t0 < t1) stage(lds0, s_coef0, t0);
         for (int t = t0; t < t1; t += 2) {
             __syncthreads();
             if (t + 1 < t1) stage(lds1, s_coef1, t + 1);
-            consume(lds0, s_coef0, t, clean_tag);
+            one(lds0, s_coef0, t);
             if (t + 1 >= t1) break;
             __syncthreads();
             if (t + 2 < t1) stage(lds0, s_coef0, t + 2);
-            consume(lds1, s_coef1, t + 1, clean_tag);
+            one(lds1, s_coef1, t + 1);
         }
     };
-    pass(std::false_type{});
+    // two products and dz side by side
+    auto pass = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) acc[x] = {};
+        if (t0 >= t1) return;
+        Pieces<T> dz = {};                                             // of the tile before, whose rows are in lds3 at the start
+        for (int i = threadIdx.x * 16; i < L::BYTES; i += 4096) *(u32x4*)(lds3 + i) = u32x4{0, 0, 0, 0};
+        stage(lds0, s_coef0, t0);
+        if (t0 + 1 < t1) stage(lds1, s_coef1, t0 + 1);
+        __syncthreads();
+        f32x16_t pr = products<T, CP>(lds0, q, lane);
+        auto step = [&](int t, const char* before, const char* here, const char* next, char* after, const float (*coef)[64],
+                        float (*coef_after)[64]) __attribute__((always_inline)) {
+            __syncthreads();                                           // tile t + 1 is there; nobody reads tile t - 2 any more
+            stage(after, coef_after, t + 2);                           // also behind the part's last tile, to no effect: no branch
+            float wv[16];
+            load_weights(wv, t);
+            f32x16_t nxt = {};
+            Pieces<T> mine;
+            float z[16];
+            Quad k4 = quad(coef, 0), ahead_k4 = k4;
+            // One slice: a fragment is read (two slices ahead of its use), multiplied (in bf16, second product: by one of the two pieces), and a
+            // share of dz is computed: 16 values, then, in pairs, their pieces.  Weights may arrive during the first half of the slices.
+            constexpr int FRAGS = NKF + NX * Pieces<T>::STEPS, SLICES = NKF + NX * Pieces<T>::STEPS * Pieces<T>::N, UNITS = 24;
+            u32x4 f[3];
+            auto read = [&](int n) __attribute__((always_inline)) {
+                if (n < NKF) f[n % 3] = row_fragment<T, CP>(next, n, lane);
+                else if (n < FRAGS) f[n % 3] = column_fragment<T, CP>(before, (n - NKF) / NX, (n - NKF) % NX * 32, lane, false);
+            };
+            read(0);
+            read(1);
+#pragma unroll
+            for (int i = 0; i < SLICES; ++i) {
+                const int n = i < NKF ? i : NKF + (i - NKF) / Pieces<T>::N, piece = i < NKF ? 0 : (i - NKF) % Pieces<T>::N;
+                if (piece == 0) {
+                    read(n + 2);
+                    settle(f[n % 3]);
+                }
+                if (n < NKF) Wide<T>::run(nxt, f[n % 3], q[n < NKF ? n : 0]);
+                else Wide<T>::run(acc[n < NKF ? 0 : (n - NKF) % NX], f[n % 3], dz.p[n < NKF ? 0 : (n - NKF) / NX][piece]);
+                const int from = GENERAL ? (2 * i < SLICES ? 0 : (2 * i - SLICES) * UNITS / SLICES) : i * UNITS / SLICES;
+                const int to = GENERAL ? (2 * i + 2 < SLICES ? 0 : (2 * i + 2 - SLICES) * UNITS / SLICES) : (i + 1) * UNITS / SLICES;
+#pragma unroll
+                for (int u = from; u < to; ++u) {
+                    if (u < 16) {
+                        if (u % 4 == 0 && u > 0) k4 = ahead_k4;
+                        if (OWN_BANK && u % 4 == (F32 ? 3 : 0) && u < 12) ahead_k4 = quad(coef, u / 4 + 1);
+                        z[u] = differentiate(pr, wv, k4, u, t, std::false_type{});
+                        settle(z[u]);
+                    } else {
+                        mine.pair(u - 16, z[2 * (u - 16)], z[2 * (u - 16) + 1]);
+                        mine.settle_pair(u - 16);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            pr = nxt;
+            dz = mine;
+            add_targets(here, coef, t, false);
+        };
+        int t = t0;                                                    // no way out of the loop's middle: it would cost copies of the sums
+        for (; t + 4 <= t1; t += 4) {
+            step(t, lds3, lds0, lds1, lds2, s_coef0, s_coef2);
+            step(t + 1, lds0, lds1, lds2, lds3, s_coef1, s_coef3);
+            step(t + 2, lds1, lds2, lds3, lds0, s_coef2, s_coef0);
+            step(t + 3, lds2, lds3, lds0, lds1, s_coef3, s_coef1);
+        }
+        if (t < t1) step(t, lds3, lds0, lds1, lds2, s_coef0, s_coef2);
+        if (t + 1 < t1) step(t + 1, lds0, lds1, lds2, lds3, s_coef1, s_coef3);
+        if (t + 2 < t1) step(t + 2, lds1, lds2, lds3, lds0, s_coef2, s_coef0);
+        const int last = (t1 - 1 - t0) & 3;
+        second_product<T, CP>(acc, last == 0 ? lds0 : last == 1 ? lds1 : last == 2 ? lds2 : lds3, dz, lane, false);
+    };
+    if constexpr (CP <= 128) pass();
+    else plain_pass(std::false_type{});
     bool broken = false;
 #pragma unroll
-    for (int x = 0; x < CP / 32; ++x)
+    for (int x = 0; x < NX; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) broken |= !(__builtin_fabsf(acc[x][i]) <= FLT_MAX);
     if (threadIdx.x == 0) s_again = 0;
     __syncthreads();                                                   // also: nobody reads the tiles any more
     if (broken) s_again = 1;
     __syncthreads();
-    if (s_again) pass(std::true_type{});
+    if (s_again) plain_pass(std::true_type{});
     if (!live) return;
+    if (!OWN_BANK && part == 0) {
+        const int target = __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + own]);
+        const float gl = a.coef[K_LOGP * n_coef + own];
+        if (target >= 0 && !(GENERAL && w && w[target] == __builtin_inff())) {
+            const T* row = (const T*)a.other + (size_t)target * a.ld_other;
 #pragma unroll
-    for (int x = 0; x < CP / 32; ++x)
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int ch = x * 32 + 8 * (i >> 2) + 4 * g + (i & 3);
+                    if (ch < a.channels) acc[x][i] += gl * to_f32(row[ch]);
+                }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int ch = x * 32 + 8 * b + 4 * g;
@@ -274,7 +383,7 @@ __global__ __launch_bounds__(256) void bank_gradient_join_kernel(BankArgs a, int
 
 
 template <typename T, int CP>
-static void launch_gradient(const BankArgs& a, bool own_bank, hipStream_t st) {
+static void launch(const BankArgs& a, bool own_bank, hipStream_t st) {
     const dim3 grid((unsigned)((a.n_own + 127) / 128 * a.parts));
     const bool general = a.out.k == 0.0f;
     if (own_bank) {
@@ -288,26 +397,12 @@ static void launch_gradient(const BankArgs& a, bool own_bank, hipStream_t st) {
         hipLaunchKernelGGL((bank_gradient_join_kernel<T>), dim3((unsigned)(((long)a.n_own * a.channels + 255) / 256)), dim3(256), 0, st, a, CP);
 }
 
-template <typename T>
-static void launch_gradient(const BankArgs& a, bool own_bank, hipStream_t st) {
+template <> void launch_bank_gradient<NEMO_ELEMENT>(const BankArgs& a, bool own_bank, hipStream_t st) {
     switch (padded_channels(a.channels)) {
-        case 32: launch_gradient<T, 32>(a, own_bank, st); break;
-        case 64: launch_gradient<T, 64>(a, own_bank, st); break;
-        case 128: launch_gradient<T, 128>(a, own_bank, st); break;
-        default: launch_gradient<T, 256>(a, own_bank, st);
+        case 64: launch<NEMO_ELEMENT, 64>(a, own_bank, st); break;
+        case 128: launch<NEMO_ELEMENT, 128>(a, own_bank, st); break;
+        default: launch<NEMO_ELEMENT, 256>(a, own_bank, st);
     }
-}
-
-
-void launch_bank_gradient(const BankArgs& a, int dtype, bool own_bank, hipStream_t st) {
-    if (dtype == NEMO_F32) launch_gradient<float>(a, own_bank, st);
-    else launch_gradient<bf16>(a, own_bank, st);
-}
-
-void launch_bank_coef(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse, const long long* targets, int rows,
-                      int cols, float* coef, bool join_m, hipStream_t st) {
-    hipLaunchKernelGGL(bank_coef_kernel, dim3((unsigned)((coef_rows(rows) + 255) / 256)), dim3(256), 0, st, stats, g_logp, g_entropy, g_lse,
-                       targets, rows, cols, coef, join_m);
 }
 
 }  // namespace nemo

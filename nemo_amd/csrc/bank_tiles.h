@@ -1,4 +1,4 @@
-// What the kernels of bank_log_probs.hip and bank_gradient.hip share: arguments, tiles in LDS, the first product.
+// What the kernels of bank_forward.hip and bank_gradient.hip share: arguments, tiles in LDS, the first product.
 //
 // 32 "owner" rows, whose fragments a wave keeps in registers, are multiplied with tiles of "other" rows that the workgroup's four waves share in
 // LDS (two buffers, copied from global memory without registers), on v_mfma_f32_32x32x{16 bf16, 2 f32} with the other rows as first operand.
@@ -46,39 +46,56 @@ struct BankArgs {
     void* grad;                    // [n_own][channels]
 };
 
-// A tile in LDS.  Each instruction of a copy writes 1024 bytes, RPI rows; rows of 256 bytes and more get 16 RPI bytes of padding behind them, and
-// chunk c of row r lies at c ^ flip(r) within its row: rows that one LDS read touches at the same chunk then lie in different banks.  flip
-// reaches the lowest bits of a chunk index only, so that the addresses of a lane differ by constants, which need no registers.
+// A tile of 32 rows in LDS.  Each instruction of a copy writes 1024 bytes, RPI rows, and 16 bytes of padding are left behind them; chunk c (16 bytes)
+// of row r lies at c ^ flip(r) within its row.  Padding and flip put what one LDS read touches into different banks: the same chunk of 16
+// consecutive rows (row_fragment), and 64 bytes of four consecutive rows (the transposing reads of the second product).  flip reaches the
+// bits MASK of a chunk index only, so that most addresses of a lane differ by constants, which need no registers.
 template <typename T, int CP> struct Tile {
-    static constexpr int RB = CP * (int)sizeof(T), CPR = RB / 16, RPI = 1024 / RB, PITCH = 1024 + (RB >= 256 ? 16 * RPI : 0);
-    static constexpr int MASK = RPI >= 16 ? 3 : RPI - 1;               // chunk bits that flip reaches
-    static constexpr int ROWS = RB >= 1024 ? 32 : 64;                  // rows of a tile
-    static constexpr int BYTES = ROWS / RPI * PITCH;
-    static __device__ constexpr int flip(int r) { return RPI >= 16 ? (r >> 1) & 3 : r & MASK; }
+    static constexpr int RB = CP * (int)sizeof(T), CPR = RB / 16, RPI = 1024 / RB, PITCH = 1024 + (RB >= 128 ? 16 : 0);
+    static constexpr int MASK = RPI == 16 ? 3 : RPI == 8 ? 7 : RPI == 4 ? 12 : RPI == 2 ? 8 : 0;
+    static constexpr int ROWS = 32, COPIES = ROWS / RPI, BYTES = COPIES * PITCH;
+    static __device__ constexpr int flip(int r) {
+        return RPI == 16 ? (r >> 2) & 3 : RPI == 8 ? r & 7 : RPI == 4 ? (r & 3) << 2 : RPI == 2 ? (r & 1) << 3 : 0;
+    }
     static __device__ constexpr int row(int r) { return r / RPI * PITCH + r % RPI * RB; }
+    // Byte offset of chunk a + b (no bit in common; a a constant) in a row whose flip is f.
+    static __device__ constexpr int chunk(int a, int b, int f) { return ((((a & MASK) | (b & MASK)) ^ f) + (a & ~MASK) + (b & ~MASK)) << 4; }
 };
 
-template <typename T, int CP>
-__device__ inline void stage_rows(char* lds, const T* base, long ld, int row0, int rows, int channels, int wave, int lane) {
+// What a lane copies of every tile: its chunk of row `row` of the tile, or zeros (rows beyond the last, channels beyond the last).
+template <typename T, int CP> struct Stager {
     typedef Tile<T, CP> L;
-    constexpr int EPC = 16 / (int)sizeof(T);
-    static_assert(L::ROWS / L::RPI % 4 == 0, "every wave copies the same number of kilobytes");
+    static constexpr int N = (L::COPIES + 3) / 4;                      // copies of a wave
+    const T* src[N];
+    int row[N];
+    long step;                                                         // elements from tile to tile
+    int rows, wave;
+    __device__ inline Stager(const T* base, long ld, int rows_, int channels, int wave_, int lane) : step(32 * ld), rows(rows_), wave(wave_) {
+        constexpr int EPC = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < L::ROWS / L::RPI / 4; ++i) {
-        const int j = i * 4 + wave;
-        const int r = j * L::RPI + lane / L::CPR, c = (lane & (L::CPR - 1)) ^ L::flip(r);
-        const bool in = row0 + r < rows && c * EPC < channels;
-        const T* src = base + (size_t)(row0 + r) * ld + c * EPC;
-        copy_to_lds(in ? (const void*)src : (const void*)&g_zero_row, lds + j * L::PITCH);
+        for (int i = 0; i < N; ++i) {
+            const int r = (i * 4 + wave) * L::RPI + lane / L::CPR, c = (lane & (L::CPR - 1)) ^ L::flip(r);
+            src[i] = base + (long)r * ld + c * EPC;
+            row[i] = c * EPC < channels ? r : 0x40000000;
+        }
     }
-}
+    __device__ inline void copy(char* lds, int tile) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = i * 4 + wave;
+            if (L::COPIES % 4 && j >= L::COPIES) break;
+            const T* p = src[i] + (long)tile * step;
+            copy_to_lds(tile * 32 + row[i] < rows ? (const void*)p : (const void*)&g_zero_row, lds + j * L::PITCH);
+        }
+    }
+};
 
-// Fragment kf of the 32 rows that start at `row` (a multiple of 32).
+// Fragment kf of the tile's rows.
 template <typename T, int CP>
-__device__ inline u32x4 row_fragment(const char* lds, int row, int kf, int lane) {
+__device__ inline u32x4 row_fragment(const char* lds, int kf, int lane) {
     typedef Tile<T, CP> L;
-    const int r = lane & 31, low = ((2 * kf) & L::MASK) + (lane >> 5);
-    return *(const u32x4*)(lds + L::row(row) + (((2 * kf) & ~L::MASK) << 4) + L::row(r) + ((low ^ L::flip(r)) << 4));
+    const int r = lane & 31;
+    return *(const u32x4*)(lds + L::row(r) + L::chunk(2 * kf, lane >> 5, L::flip(r)));
 }
 
 // Fragment of owner rows straight from memory.
@@ -95,22 +112,26 @@ __device__ inline void own_fragments(u32x4 (&q)[CP / Wide<T>::KF], const BankArg
     }
 }
 
-// The compiler would read all fragments ahead and run out of registers: it may not look further ahead than `AHEAD` of them.
 template <typename T, int CP>
-__device__ inline f32x16_t products(const char* lds, int row, const u32x4 (&q)[CP / Wide<T>::KF], int lane) {
-    constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;
+__device__ inline f32x16_t products(const char* lds, const u32x4 (&q)[CP / Wide<T>::KF], int lane) {
+    constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;                      // fragments that may be read ahead: registers
     f32x16_t acc = {};
 #pragma unroll
     for (int kf = 0; kf < CP / Wide<T>::KF; ++kf) {
-        Wide<T>::run(acc, row_fragment<T, CP>(lds, row, kf, lane), q[kf]);
+        Wide<T>::run(acc, row_fragment<T, CP>(lds, kf, lane), q[kf]);
         if (kf % AHEAD == AHEAD - 1) __builtin_amdgcn_sched_barrier(0);
     }
     return acc;
 }
 
+// Keeps the compiler from moving the computation of x behind this point (it would put it where x is used, out of reach of the matrix
+// instructions that it is meant to run beside).
+__device__ inline void settle(u32x4& x) { asm volatile("" : "+v"(x)); }
+__device__ inline void settle(float& x) { asm volatile("" : "+v"(x)); }
+
 struct __attribute__((packed, aligned(4))) LooseQuad { f32x4 v; };
 
-// Weights of the lane's 16 other rows j0 + 8 b + 4 g + i, 0 beyond `end`; w: the row of weights of the lane's feature row.
+// Weights of the lane's 16 other rows j0 + 8 b + 4 g + i, +inf (left out) beyond `end`; w: the row of weights of the lane's feature row.
 __device__ inline void row_weights(float wv[16], const float* w, int j0, int g, int end) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -121,20 +142,23 @@ __device__ inline void row_weights(float wv[16], const float* w, int j0, int g, 
             for (int i = 0; i < 4; ++i) wv[4 * b + i] = q[i];
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) wv[4 * b + i] = j + i < end ? w[j + i] : 0.0f;
+            for (int i = 0; i < 4; ++i) wv[4 * b + i] = j + i < end ? w[j + i] : __builtin_inff();
         }
     }
 }
 
 
-void launch_bank_gradient(const BankArgs& a, int dtype, bool own_bank, hipStream_t st);
-void launch_bank_coef(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse, const long long* targets, int rows,
-                      int cols, float* coef, bool join_m, hipStream_t st);
+template <typename T> void launch_bank_forward(const BankArgs& a, hipStream_t st);
+template <typename T> void launch_bank_gradient(const BankArgs& a, bool own_bank, hipStream_t st);
+template <> void launch_bank_forward<float>(const BankArgs& a, hipStream_t st);
+template <> void launch_bank_forward<bf16>(const BankArgs& a, hipStream_t st);
+template <> void launch_bank_gradient<float>(const BankArgs& a, bool own_bank, hipStream_t st);
+template <> void launch_bank_gradient<bf16>(const BankArgs& a, bool own_bank, hipStream_t st);
 
 // The six arrays that the gradient kernels need of every feature row; rows beyond the last have p = 0 and no target.
 enum { K_M, K_LOG2_S, K_C, K_G2, K_LOGP, K_TARGET, K_COUNT };
-constexpr int coef_rows(int64_t rows) { return (int)((rows + 63) / 64 * 64 + 64); }
+constexpr int coef_rows(int64_t rows) { return (int)((rows + 63) / 64 * 64 + 192); }
 
-inline int padded_channels(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : 256; }
+inline int padded_channels(int c) { return c <= 64 ? 64 : c <= 128 ? 128 : 256; }
 
 }  // namespace nemo

@@ -116,6 +116,7 @@ __device__ inline void write_top(const RowOut& o, long row, int i, const Softmax
 // The gradient of one score: with log2 p = x - log2 s,
 //     dz = p (g_lse - g_logp - g_entropy (log p + entropy)) + [j = target] g_logp = p (c - g2 log2 p) + [j = target] g_logp,
 // c = g_lse - g_logp - g_entropy entropy and g2 = g_entropy log 2.  Places that are left out get none.
+constexpr float kNoProbability = 1.0e30f;              // exp2(x - this) is 0, and 0 times it as well
 struct RowCoef { float m, log2_s, c, g2, g_logp; int target; };
 __device__ inline RowCoef row_coef(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse, const long long* targets,
                                    long row, long long cols) {
@@ -124,7 +125,7 @@ __device__ inline RowCoef row_coef(const float* stats, const float* g_logp, cons
     const float ge = g_entropy ? g_entropy[row] : 0.0f;
     RowCoef k;
     k.m = st[0];
-    k.log2_s = st[1] == neg_inf() ? __builtin_inff() : st[1];          // a row with nothing left: p = 0 everywhere
+    k.log2_s = st[1] == neg_inf() ? kNoProbability : st[1];            // a row with nothing left: p = 0 everywhere
     k.g2 = ge * kLn2;
     k.g_logp = g_logp && t >= 0 && t < cols ? g_logp[row] : 0.0f;
     k.c = (g_lse ? g_lse[row] : 0.0f) - k.g_logp - ge * st[2];
