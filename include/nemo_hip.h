@@ -484,14 +484,15 @@ int nemo_bank_log_probs(const void* features, int64_t ldf, const void* bank, int
                         void* workspace, size_t workspace_bytes, void* stream);
 /* With dz as nemo_log_probs_backward has it (without its factor scale):
  *   grad_features[i] = scale sum_j dz[i,j] bank[j],   grad_bank[j] = scale sum_i dz[i,j] features[i]
- * (contiguous, element type dtype; NULL: not wanted).  The scores are computed again.  Places that are left out add nothing, whatever the
+ * (contiguous, element type dtype; NULL: not wanted).  weights, scale and top as in the call that wrote `stats` (they decide the form in
+ * which it is kept).  The scores are computed again.  Places that are left out add nothing, whatever the
  * feature or bank row holds.  Sums run in a fixed order: two calls give the same bits. */
 size_t nemo_bank_log_probs_backward_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                               int64_t channels, int32_t dtype);
 int nemo_bank_log_probs_backward(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,
                                  const int64_t* targets, const float* stats, const float* g_logp, const float* g_entropy,
                                  const float* g_lse, int64_t rows, int64_t cols, int64_t channels, int32_t dtype, float scale,
-                                 void* grad_features, void* grad_bank, void* workspace, size_t workspace_bytes, void* stream);
+                                 int32_t top, void* grad_features, void* grad_bank, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -123,8 +123,8 @@ def load():
     lib.nemo_bank_log_probs_workspace.argtypes = [vp, i64, vp, i64, i64, i64, i64, i32, i32]
     lib.nemo_bank_log_probs.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i32, C.c_float, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.nemo_bank_log_probs_backward_workspace.argtypes = [vp, i64, vp, i64, i64, i64, i64, i32]
-    lib.nemo_bank_log_probs_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, C.c_float, vp, vp, vp, sz,
-                                                 vp]
+    lib.nemo_bank_log_probs_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, C.c_float, i32, vp, vp, vp,
+                                                 sz, vp]
     dense_workspaces = ("nemo_linear_workspace", "nemo_linear_backward_workspace", "nemo_log_probs_workspace", "nemo_bank_log_probs_workspace",
                         "nemo_bank_log_probs_backward_workspace")
     for name in dense_workspaces:

@@ -167,7 +167,7 @@ class _BankLogProbs(torch.autograd.Function):
     def forward(ctx, features, bank, targets, weights, scale, top):
         out, stats, top_logp, top_index = ops.bank_log_probs(features, bank, targets, weights, scale, top)
         ctx.save_for_backward(features, bank, targets, weights, stats)
-        ctx.scale = scale
+        ctx.scale, ctx.top = scale, top
         if top:
             ctx.mark_non_differentiable(top_logp, top_index)
         ctx.set_materialize_grads(False)
@@ -179,7 +179,7 @@ class _BankLogProbs(torch.autograd.Function):
         features, bank, targets, weights, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:
             return (None,) * 6
-        grads = ops.bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, ctx.scale,
+        grads = ops.bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, ctx.scale, ctx.top,
                                             ctx.needs_input_grad[:2])
         return (*grads, None, None, None, None)
 

@@ -10,23 +10,23 @@
 
 namespace nemo {
 
-// Puts v into the list, ordered by v * order (the score; a score is not smaller where the product is not, but may be equal).  Places arrive
-// in rising order, so an equal score goes behind those already there.
+// Puts z into the list.  Places arrive in rising order, so an equal score goes behind those already there.  A score at least as large as entry
+// i - 1 and one between two entries are both the median of the two and z.
 template <int TOP>
-__device__ inline void insert(float (&tv)[TOP], int (&tp)[TOP], float v, int place, float order) {
-    const float z = v * order;
+__device__ inline void insert(float (&tv)[TOP], int (&tp)[TOP], float z, int place) {
+    bool above = z > tv[TOP - 1];
 #pragma unroll
-    for (int i = TOP - 1; i >= 0; --i) {
-        const bool above = z > tv[i] * order;
-        const bool shift = i > 0 && z > tv[i > 0 ? i - 1 : 0] * order;
-        if (above) {
-            tv[i] = shift ? tv[i > 0 ? i - 1 : 0] : v;
-            tp[i] = shift ? tp[i > 0 ? i - 1 : 0] : place;
-        }
+    for (int i = TOP - 1; i > 0; --i) {
+        const bool shift = z > tv[i - 1];
+        tp[i] = shift ? tp[i - 1] : above ? place : tp[i];
+        tv[i] = __builtin_amdgcn_fmed3f(z, tv[i - 1], tv[i]);
+        above = shift;
     }
+    tp[0] = above ? place : tp[0];
+    tv[0] = fmaxf(z, tv[0]);
 }
 
-// GENERAL: with weights, or with hardly any scale; see softmax_state.h for the two forms of the state.  The sign of the scale goes into the
+// GENERAL: with weights, with a list (its order is that of the scores), or with hardly any scale; see softmax_state.h for the two forms of the state.  The sign of the scale goes into the
 // owners' fragments where the state is kept of the products.
 //
 // Tiles of 32 bank rows; in step n the wave multiplies tile n + 1 while it takes the products of tile n into the state, so that matrix cores
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
     const long long tl = live ? a.targets[row] : -1;
     const int target = tl >= 0 && tl < a.n_other ? (int)tl : -1;
     const float scale = GENERAL ? a.scale : __builtin_fabsf(a.scale);
-    const float k = a.out.k, order = GENERAL ? 1.0f : scale, unit = GENERAL ? kLog2e : 1.0f;
+    const float k = a.out.k, unit = GENERAL ? kLog2e : 1.0f;
     SoftmaxState st;
     float tv[NT];
     int tp[NT];
@@ -84,13 +84,12 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
                 if (at == 8 * (i >> 2) + (i & 3)) a.z_target[row] = v[i];
         }
         if (TOP > 0) {
-            float peak = v[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) peak = fmaxf(peak, v[i]);
-            if (__any(peak * order > tv[NT - 1] * order)) {
+            // nothing below the worst entry of either list of the row belongs to its best
+            const float bar = fmaxf(tv[NT - 1], __shfl_xor(tv[NT - 1], 32));
+            if (__any(peak_of(v) > bar)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (__any(v[i] * order > tv[NT - 1] * order)) insert(tv, tp, v[i], j0 + 8 * (i >> 2) + 4 * g + (i & 3), order);
+                    if (__any(v[i] > bar)) insert(tv, tp, v[i] > bar ? v[i] : neg_inf(), j0 + 8 * (i >> 2) + 4 * g + (i & 3));
             }
         }
     };
@@ -211,17 +210,10 @@ template <typename T, int CP>
 static void launch(const BankArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.n_own + 127) / 128 * a.parts));
     const int top = a.out.top;
-    const bool general = a.out.k == 0.0f;
-    if (top == 0) {
-        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, false>), grid, dim3(256), 0, st, a);
-    } else if (top <= 5) {
-        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, false>), grid, dim3(256), 0, st, a);
-    } else {
-        if (general) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, false>), grid, dim3(256), 0, st, a);
-    }
+    if (a.out.k != 0.0f) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, false>), grid, dim3(256), 0, st, a);
+    else if (top == 0) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, true>), grid, dim3(256), 0, st, a);
+    else if (top <= 5) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, true>), grid, dim3(256), 0, st, a);
 }
 
 template <> void launch_bank_forward<NEMO_ELEMENT>(const BankArgs& a, hipStream_t st) {

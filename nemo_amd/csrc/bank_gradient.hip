@@ -121,15 +121,16 @@ template <typename T, int CP, bool OWN_BANK, bool GENERAL>
 __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(BankArgs a) {
     typedef Tile<T, CP> L;
     constexpr bool F32 = sizeof(T) == 4, SPLIT = GENERAL || F32;       // log2 s apart from m
+    constexpr bool SIDE_BY_SIDE = CP <= 128 && !(F32 && GENERAL);
     constexpr int NX = CP / 32, NKF = CP / Wide<T>::KF;
     __shared__ __attribute__((aligned(16))) char lds0[L::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[L::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds2[L::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds3[L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds2[SIDE_BY_SIDE ? L::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) char lds3[SIDE_BY_SIDE ? L::BYTES : 16];
     __shared__ __attribute__((aligned(16))) float s_coef0[OWN_BANK ? K_COUNT : 1][64];
     __shared__ __attribute__((aligned(16))) float s_coef1[OWN_BANK ? K_COUNT : 1][64];
-    __shared__ __attribute__((aligned(16))) float s_coef2[OWN_BANK ? K_COUNT : 1][64];
-    __shared__ __attribute__((aligned(16))) float s_coef3[OWN_BANK ? K_COUNT : 1][64];
+    __shared__ __attribute__((aligned(16))) float s_coef2[OWN_BANK && SIDE_BY_SIDE ? K_COUNT : 1][64];
+    __shared__ __attribute__((aligned(16))) float s_coef3[OWN_BANK && SIDE_BY_SIDE ? K_COUNT : 1][64];
     __shared__ int s_again;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int part = (int)(blockIdx.x % a.parts);
@@ -300,8 +301,9 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
 #pragma unroll
                 for (int u = from; u < to; ++u) {
                     if (u < 16) {
-                        if (u % 4 == 0 && u > 0) k4 = ahead_k4;
-                        if (OWN_BANK && u % 4 == (F32 ? 3 : 0) && u < 12) ahead_k4 = quad(coef, u / 4 + 1);
+                        // f32: no registers to read ahead, and four times the matrix instructions to wait beside
+                        if (u % 4 == 0 && u > 0) k4 = OWN_BANK && F32 ? quad(coef, u / 4) : ahead_k4;
+                        if (OWN_BANK && !F32 && u % 4 == 0 && u < 12) ahead_k4 = quad(coef, u / 4 + 1);
                         z[u] = differentiate(pr, wv, k4, u, t, std::false_type{});
                         settle(z[u]);
                     } else {
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
         const int last = (t1 - 1 - t0) & 3;
         second_product<T, CP>(acc, last == 0 ? lds0 : last == 1 ? lds1 : last == 2 ? lds2 : lds3, dz, lane, false);
     };
-    if constexpr (CP <= 128) pass();
+    if constexpr (SIDE_BY_SIDE) pass();
     else plain_pass(std::false_type{});
     bool broken = false;
 #pragma unroll

@@ -22,19 +22,13 @@ __global__ __launch_bounds__(256) void bank_join_kernel(BankArgs a) {
         const long long t = a.targets[row];
         write_row(a.out, row, st, t, a.n_other, t >= 0 && t < a.n_other ? a.z_target[row] : 0.0f);
     }
-    const float order = a.out.k == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
     int walk = 0;
     for (int i = 0; i < top; ++i) {
-        float v = neg_inf();
         Entry mine = no_entry();
-        if (lane < n && walk < top) {
-            v = a.part_z[at * top + walk];
-            mine = {v * order, a.part_place[at * top + walk]};
-        }
+        if (lane < n && walk < top) mine = {a.part_z[at * top + walk], a.part_place[at * top + walk]};
         const Entry e = wave_best(mine);
-        const bool owner = mine.place == e.place && e.place != kNoPlace;
-        if (owner) ++walk;
-        if (owner || (e.place == kNoPlace && lane == 0)) write_top(a.out, row, i, st, {v, e.place});
+        if (mine.place == e.place && mine.z == e.z) ++walk;
+        if (lane == 0) write_top(a.out, row, i, st, e);
     }
 }
 
@@ -85,10 +79,10 @@ static Parts parts_of_bank(int64_t owners, int64_t others, int per_cu) {
 static Parts forward_parts(int64_t rows, int64_t cols, int cp, int es) { return parts_of_bank(rows, cols, cp * es <= 256 ? 4 : 2); }
 static Parts gradient_parts(int64_t owners, int64_t others, int cp) { return parts_of_bank(owners, others, cp == 256 ? 1 : 2); }
 
-// The state's form: 0 with weights (or hardly any scale), else what turns a product into its score in units of log 2.
-static float product_unit(const float* weights, float scale) {
+// The state's form: 0 where it is kept of the scores, else what turns a product into its score in units of log 2.
+static float product_unit(const float* weights, float scale, int top) {
     const float s = scale < 0.0f ? -scale : scale;
-    return weights || !(s >= 1.0e-30f) ? 0.0f : s * kLog2e;
+    return weights || top > 0 || !(s >= 1.0e-30f) ? 0.0f : s * kLog2e;
 }
 
 static int check_bank(const char* who, int64_t rows, int64_t cols, int64_t channels, int dtype, int top) {
@@ -158,7 +152,7 @@ extern "C" int nemo_bank_log_probs(const void* features, int64_t ldf, const void
     a.part_place = (int*)ws;
     ws += align256((size_t)2 * p.parts * rows * top * 4);
     a.z_target = (float*)ws;
-    a.out = {out_logp, out_entropy, out_lse, out_stats, out_top_logp, (long long*)out_top_index, top, product_unit(weights, scale)};
+    a.out = {out_logp, out_entropy, out_lse, out_stats, out_top_logp, (long long*)out_top_index, top, product_unit(weights, scale, top)};
     if (dtype == NEMO_F32) launch_bank_forward<float>(a, st);
     else launch_bank_forward<bf16>(a, st);
     hipLaunchKernelGGL(bank_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
@@ -179,8 +173,8 @@ extern "C" size_t nemo_bank_log_probs_backward_workspace(const void* features, i
 extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,
                                             const int64_t* targets, const float* stats, const float* g_logp, const float* g_entropy,
                                             const float* g_lse, int64_t rows, int64_t cols, int64_t channels, int32_t dtype, float scale,
-                                            void* grad_features, void* grad_bank, void* workspace, size_t workspace_bytes, void* stream) {
-    int rc = check_bank("nemo_bank_log_probs_backward", rows, cols, channels, dtype, 0);
+                                            int32_t top, void* grad_features, void* grad_bank, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_bank("nemo_bank_log_probs_backward", rows, cols, channels, dtype, top);
     if (rc) return rc;
     if (rows == 0 || cols == 0) return NEMO_OK;
     if (!features || !bank || !targets || !stats) return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs_backward: null argument");
@@ -196,7 +190,7 @@ extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, c
     const RowsIn f = rows_in(dtype, features, ldf, rows, channels, ws, st), b = rows_in(dtype, bank, ldb, cols, channels, ws, st);
     float* coef = (float*)ws;
     ws += align256((size_t)K_COUNT * coef_rows(rows) * 4);
-    const float unit = product_unit(weights, scale);
+    const float unit = product_unit(weights, scale, top);
     hipLaunchKernelGGL(bank_coef_kernel, dim3((unsigned)((coef_rows(rows) + 255) / 256)), dim3(256), 0, st, stats, g_logp, g_entropy, g_lse,
                        (const long long*)targets, (int)rows, (int)cols, coef, unit != 0.0f && dtype == NEMO_BF16);
     const int cp = padded_channels((int)channels);

@@ -36,7 +36,7 @@ struct BankArgs {
     int parts, part_tiles;         // tiles of other rows a part
     // forward
     float* part_state;             // [3][2 parts][rows]
-    float* part_z;                 // [2 parts][rows][top]: products (scores where out.k = 0) in the order of their scores
+    float* part_z;                 // [2 parts][rows][top]
     int* part_place;
     float* z_target;               // [rows]
     RowOut out;

@@ -831,8 +831,8 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
     return out, stats, top_logp, top_index
 
 
-def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0, want=(True, True)):
-    """-> (grad_features, grad_bank), None where `want` is false."""
+def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0, top=0, want=(True, True)):
+    """-> (grad_features, grad_bank), None where `want` is false; weights, scale and top as in the call that gave `stats`."""
     lib = _lib.load()
     (S, ch), V = features.shape, bank.shape[0]
     features, ldf = rows_2d(features, ch)
@@ -847,6 +847,6 @@ def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_e
         nbytes = lib.nemo_bank_log_probs_backward_workspace(_raw(features), ldf, _raw(bank), ldb, S, V, ch, dt)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_bank_log_probs_backward(_raw(features), ldf, _raw(bank), ldb, _raw(weights), ldw, _raw(targets), _raw(stats),
-                                               *[_raw(g) for g in gs], S, V, ch, dt, float(scale), *[_raw(g) for g in grads], _raw(ws),
+                                               *[_raw(g) for g in gs], S, V, ch, dt, float(scale), int(top), *[_raw(g) for g in grads], _raw(ws),
                                                nbytes, stream_ptr()), "nemo_bank_log_probs_backward")
     return tuple(grads)

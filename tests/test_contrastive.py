@@ -790,8 +790,8 @@ def test_entry_refusals():
     assert bank(S=-1) == -1 and bank(ch=0) == -1 and bank(ch=257, ldf=257, ldb=257) == -2 and bank(dt=2) == -2 and bank(top=17) == -2
     assert bank(f=None) == -1 and bank(t=None) == -1 and bank(ldf=15) == -1 and bank(S=1 << 24) == -2 and bank(S=0) == 0
     assert bank() == -1 and "workspace" in err()
-    assert lib.nemo_bank_log_probs_backward(p, 16, p, 16, None, 0, p, None, None, None, None, 4, 9, 16, 0, 1.0, p, p, None, 0, None) == -1
-    assert lib.nemo_bank_log_probs_backward(p, 16, p, 16, None, 0, p, p, None, None, None, 4, 9, 16, 0, 1.0, p, p, None, 0, None) == -1
+    assert lib.nemo_bank_log_probs_backward(p, 16, p, 16, None, 0, p, None, None, None, None, 4, 9, 16, 0, 1.0, 0, p, p, None, 0, None) == -1
+    assert lib.nemo_bank_log_probs_backward(p, 16, p, 16, None, 0, p, p, None, None, None, 4, 9, 16, 0, 1.0, 0, p, p, None, 0, None) == -1
     assert lib.nemo_linear_workspace(p, 8, p, 8, 4, 4, 8, 0) == 0       # aligned rows and enough tiles' worth of nothing to split
 
 
