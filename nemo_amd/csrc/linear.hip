@@ -19,6 +19,7 @@
 // into the workspace with padded rows (pack_kernel).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "../../include/nemo_hip.h"
 #include "dense.h"
@@ -30,25 +31,39 @@ __device__ const u32x4 g_zero_chunk = {0, 0, 0, 0};                    // what t
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 
-__device__ inline float activate(float z, int act) {
+// erfc(a), a >= 0, to 1.5e-7: the rational approximation 7.1.26 of Abramowitz and Stegun, a quarter of erff's instructions.  For the 16-bit types, whose
+// own rounding is 2^-11 at best; f32 takes erff.
+__device__ inline float erfc_short(float a) {
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return p * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
+}
+// Standard normal distribution function at z.
+template <typename T> __device__ inline float normal_cdf(float z) {
+    if constexpr (sizeof(T) == 4) return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    const float half = 0.5f * erfc_short(__builtin_fabsf(z) * 0.70710678118654752f);
+    return z < 0.0f ? half : 1.0f - half;
+}
+template <typename T> __device__ inline float logistic(float z) {
+    if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+}
+
+template <typename T> __device__ inline float activate(float z, int act) {
     switch (act) {
         case ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-        case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case ACT_SILU: return z / (1.0f + expf(-z));
+        case ACT_GELU: return z * normal_cdf<T>(z);
+        case ACT_SILU: return z * logistic<T>(z);
         default: return z;
     }
 }
 
-// d act / d z.  relu's slope at 0 is 0.  For large negative z: gelu's exp(-z^2 / 2) underflows to 0 and silu's s to 0, for large
-// positive ones 1 + z (1 - s) is 1 because 1 - s is written as the sigmoid of -z.
-__device__ inline float activate_slope(float z, int act) {
+// d act / d z.  relu's slope at 0 is 0.  Far out gelu's exp(-z^2 / 2) and silu's s underflow to 0; 1 - s is taken as the function of -z.
+template <typename T> __device__ inline float activate_slope(float z, int act) {
     switch (act) {
         case ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-        case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-        case ACT_SILU: {
-            const float s = 1.0f / (1.0f + expf(-z)), r = 1.0f / (1.0f + expf(z));
-            return s * (1.0f + z * r);
-        }
+        case ACT_GELU: return normal_cdf<T>(z) + z * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z) * 0.39894228040143268f;
+        case ACT_SILU: return logistic<T>(z) * (1.0f + z * logistic<T>(-z));
         default: return 1.0f;
     }
 }
@@ -70,7 +85,7 @@ struct GemmArgs {
     const void* Q;
     long ldp, ldq;             // elements
     int np, nq, nk;
-    int tiles_p, tiles_q, splits, k_split;         // k_split: k of one split, whole steps
+    int big, tiles_p, tiles_q, splits, k_split;    // side of a tile; k of one split, whole steps
     float* partial;            // [splits][nq][np4] when splits > 1
     int np4;
     Epilogue e;
@@ -131,7 +146,7 @@ __device__ inline void epilogue4(const Epilogue& e, const float v[4], int q, int
     }
     if (e.act != ACT_NONE) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = activate(z[i], e.act);
+        for (int i = 0; i < 4; ++i) z[i] = activate<T>(z[i], e.act);
     }
     if (res) {
 #pragma unroll
@@ -155,33 +170,50 @@ template <int CPR> __device__ inline int swizzle_t(int k) { return (2 * (((k >> 
 
 template <typename T> constexpr int kstep() { return 128 / (int)sizeof(T); }
 
-// A tile of ROWS rows x 128 bytes of k into `lds` by WAVES waves.
-template <typename T, int ROWS, bool TR, int WAVES>
-__device__ inline void stage(char* lds, const T* base, long ld, int row0, int rows, int k0, int nk, int wave, int lane) {
-    constexpr int EPC = 16 / (int)sizeof(T);                           // elements of a chunk
-    constexpr int CHUNKS = ROWS * 8;
-    static_assert(CHUNKS % (64 * WAVES) == 0, "every wave copies the same number of kilobytes");
-#pragma unroll
-    for (int i = 0; i < CHUNKS / 64 / WAVES; ++i) {
-        const int j = i * WAVES + wave, idx = j * 64 + lane;
-        const T* src;
-        bool in;
-        if (!TR) {
-            const int r = idx >> 3, c = (idx & 7) ^ (r & 7);
-            const int row = min(row0 + r, rows - 1), k = k0 + c * EPC;
-            in = k < nk;
-            src = base + (size_t)row * ld + k;
-        } else {
-            constexpr int CPR = ROWS / EPC;
-            const int kr = idx / CPR;
-            const int c = (idx & (CPR - 1)) ^ (sizeof(T) == 2 ? swizzle_t<CPR>(kr) : 0);
-            const int col = row0 + c * EPC, k = k0 + kr;
-            in = k < nk && col < rows;
-            src = base + (size_t)k * ld + col;
-        }
-        copy_to_lds(in ? (const void*)src : (const void*)&g_zero_chunk, lds + j * 1024);
+// What a lane copies of every tile of ROWS rows x 128 bytes of k, WAVES waves sharing the work: 32-bit offsets from an address that all lanes share and
+// that moves on from tile to tile.  Rows beyond the last are replaced by the last one (their results are not stored).
+template <typename T, int ROWS, bool TR, int WAVES> struct Copier {
+    static constexpr int EPC = 16 / (int)sizeof(T), N = ROWS * 8 / 64 / WAVES, BK = kstep<T>();
+    static_assert(N * 64 * WAVES == ROWS * 8, "every wave copies the same number of kilobytes");
+    const char* base;                      // of the tile's first row (TR: first column), k = 0
+    long step;                             // bytes from tile to tile
+    uint32_t off[N];
+    int wave, lane;
+    // k of copy i within the tile
+    __device__ inline int k_of(int i) const {
+        const int idx = (i * WAVES + wave) * 64 + lane, r = idx >> 3;
+        return TR ? idx / (ROWS / EPC) : ((idx & 7) ^ (r & 7)) * EPC;
     }
-}
+    __device__ inline Copier(const void* m, long ld, int row0, int rows, int wave_, int lane_) : wave(wave_), lane(lane_) {
+        base = (const char*)m + (TR ? (long)row0 : (long)row0 * ld) * (long)sizeof(T);
+        step = (TR ? BK * ld : BK) * (long)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int idx = (i * WAVES + wave) * 64 + lane;
+            if (!TR) {
+                const int r = idx >> 3, c = (idx & 7) ^ (r & 7);
+                off[i] = (uint32_t)(min(r, rows - 1 - row0) * (int)ld + c * EPC) * (uint32_t)sizeof(T);
+            } else {
+                constexpr int CPR = ROWS / EPC;
+                const int kr = idx / CPR, c = (idx & (CPR - 1)) ^ (sizeof(T) == 2 ? swizzle_t<CPR>(kr) : 0);
+                off[i] = (uint32_t)(kr * (int)ld + min(c * EPC, (rows - 1 - row0) / EPC * EPC)) * (uint32_t)sizeof(T);
+            }
+        }
+    }
+    // Tile number t.
+    __device__ inline void copy(char* lds, int t) const {
+        const char* tile = base + (long)t * step;
+#pragma unroll
+        for (int i = 0; i < N; ++i) copy_to_lds(tile + off[i], lds + (i * WAVES + wave) * 1024);
+    }
+    // Tile number t, of which k below `left` exists; the rest is zero.
+    __device__ inline void copy_part(char* lds, int t, int left) const {
+        const char* tile = base + (long)t * step;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            copy_to_lds(k_of(i) < left ? (const void*)(tile + off[i]) : (const void*)&g_zero_chunk, lds + (i * WAVES + wave) * 1024);
+    }
+};
 
 // Fragment kf (of the tile's 128 bytes of k) of the FR rows that start at `row`.
 template <typename T, int ROWS, bool TR>
@@ -210,11 +242,14 @@ __device__ inline u32x4 fragment(const char* lds, int row, int kf, int lane) {
     }
 }
 
+// The tile of a step is multiplied in two halves of its k.  Both halves' fragments are in registers before the barrier that frees the tile's
+// buffer; behind it, while the second half is multiplied, the tile after the next one is copied into that buffer and the first half of the
+// next tile is read.  So the matrix cores have work across the barrier, and a copy has a whole step to arrive.
 template <typename T, int BP, int BQ, int WP, int WQ, bool PT, bool QT>
-__global__ __launch_bounds__(64 * WP * WQ, 2) void gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     typedef Mma<T> M;
     constexpr int WAVES = WP * WQ, TP = BP / WP, TQ = BQ / WQ, NP = TP / M::FR, NQ = TQ / M::FR;
-    constexpr int BK = kstep<T>(), NKF = BK / M::KF;
+    constexpr int BK = kstep<T>(), HALF = BK / M::KF / 2;               // fragments of k in half a tile
     __shared__ __attribute__((aligned(16))) char lds0[(BP + BQ) * 128];
     __shared__ __attribute__((aligned(16))) char lds1[(BP + BQ) * 128];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -235,62 +270,141 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm_kernel(GemmArgs a) {
     const int in = id - group * GROUP * a.tiles_p;
     const int q0 = (first + in % size) * BQ, p0 = (in / size) * BP;
 
-    const int k_begin = split * a.k_split, k_end = min(a.nk, k_begin + a.k_split);
-    const T* P = (const T*)a.P;
-    const T* Q = (const T*)a.Q;
+    const int k_begin = split * a.k_split, k_end = min(a.nk, k_begin + a.k_split), nt = (k_end - k_begin + BK - 1) / BK;
     typename M::Acc acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[i][j] = {};
 
-    auto load = [&](char* lds, int k) {
-        stage<T, BP, PT, WAVES>(lds, P, a.ldp, p0, a.np, k, k_end, wave, lane);
-        stage<T, BQ, QT, WAVES>(lds + BP * 128, Q, a.ldq, q0, a.nq, k, k_end, wave, lane);
-    };
-    auto multiply = [&](const char* lds) {
+    if (nt > 0) {
+        const Copier<T, BP, PT, WAVES> cp(a.P, a.ldp, p0, a.np, wave, lane);
+        const Copier<T, BQ, QT, WAVES> cq(a.Q, a.ldq, q0, a.nq, wave, lane);
+        const int t0 = k_begin / BK;
+        const int full = (k_end - k_begin) / BK;                       // tiles that are not cut short
+        auto load = [&](char* lds, int t) __attribute__((always_inline)) {
+            cp.copy(lds, t0 + t);
+            cq.copy(lds + BP * 128, t0 + t);
+        };
+        auto load_any = [&](char* lds, int t) __attribute__((always_inline)) {
+            if (t < full) {
+                load(lds, t);
+            } else if (t < nt) {
+                cp.copy_part(lds, t0 + t, k_end - k_begin - t * BK);
+                cq.copy_part(lds + BP * 128, t0 + t, k_end - k_begin - t * BK);
+            }
+        };
+        u32x4 pf[2][HALF][NP], qf[2][HALF][NQ];
+        // Fragment n of the HALF (NP + NQ) of half h.
+        auto read = [&](const char* lds, int h, int n) __attribute__((always_inline)) {
+            const int f = n / (NP + NQ), i = n % (NP + NQ);
+            if (i < NP) pf[h][f][i < NP ? i : 0] = fragment<T, BP, PT>(lds, wp * TP + i * M::FR, h * HALF + f, lane);
+            else qf[h][f][i < NP ? 0 : i - NP] = fragment<T, BQ, QT>(lds + BP * 128, wq * TQ + (i - NP) * M::FR, h * HALF + f, lane);
+        };
+        // Multiplies half h and, in between, reads half o of the tile in `lds`: a few fragments beside each row of products.
+        auto multiply = [&](int h, const char* lds, int o) __attribute__((always_inline)) {
+            constexpr int ROWS = HALF * NP, FRAGS = HALF * (NP + NQ);
 #pragma unroll
-        for (int kf = 0; kf < NKF; ++kf) {
-            u32x4 pf[NP], qf[NQ];
+            for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) pf[i] = fragment<T, BP, PT>(lds, wp * TP + i * M::FR, kf, lane);
+                for (int n = r * FRAGS / ROWS; n < (r + 1) * FRAGS / ROWS; ++n) read(lds, o, n);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) qf[j] = fragment<T, BQ, QT>(lds + BP * 128, wq * TQ + j * M::FR, kf, lane);
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-#pragma unroll
-                for (int j = 0; j < NQ; ++j) M::run(acc[i][j], pf[i], qf[j]);
-        }
-    };
-
-    if (k_begin < k_end) load(lds0, k_begin);
-    for (int k = k_begin; k < k_end; k += 2 * BK) {
-        __syncthreads();                                               // the tile in lds0 is there, lds1 is free
-        if (k + BK < k_end) load(lds1, k + BK);
-        multiply(lds0);
-        if (k + BK >= k_end) break;
+                for (int j = 0; j < NQ; ++j) M::run(acc[r % NP][j], pf[h][r / NP][r % NP], qf[h][r / NP][j]);
+                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto step = [&](char* here, const char* next, int t, auto any_tag) __attribute__((always_inline)) {
+            multiply(0, here, 1);
+            __syncthreads();                                           // the next tile is there, nobody reads this one any more
+            if constexpr (decltype(any_tag)::value) load_any(here, t + 2);
+            else load(here, t + 2);
+            multiply(1, next, 0);                                      // behind the last tile what is read is of no use, and none is made of it
+        };
+        load_any(lds0, 0);
+        load_any(lds1, 1);
         __syncthreads();
-        if (k + 2 * BK < k_end) load(lds0, k + 2 * BK);
-        multiply(lds1);
+#pragma unroll
+        for (int n = 0; n < HALF * (NP + NQ); ++n) read(lds0, 0, n);
+        int t = 0;
+        for (; t + 3 < full; t += 2) {                                 // straight code: no tile that is cut short, none missing
+            step(lds0, lds1, t, std::false_type{});
+            step(lds1, lds0, t + 1, std::false_type{});
+        }
+        for (; t < nt; t += 2) {
+            step(lds0, lds1, t, std::true_type{});
+            if (t + 1 < nt) step(lds1, lds0, t + 1, std::true_type{});
+        }
     }
 
     const int g = lane / M::FR;
+    constexpr int QUADS = NP * M::QUADS;                                // quads of columns of a lane
+    auto column = [&](int n) __attribute__((always_inline)) { return p0 + wp * TP + n / M::QUADS * M::FR + n % M::QUADS * 8 + 4 * g; };
+    auto quad = [&](int n, int j) __attribute__((always_inline)) {
+        const typename M::Acc& c = acc[n / M::QUADS][j];
+        const int b = n % M::QUADS;
+        return (f32x4){c[4 * b], c[4 * b + 1], c[4 * b + 2], c[4 * b + 3]};
+    };
+    if (a.splits == 1 && a.e.vec) {
+        // bias once, a row's residual all at once, the next row's while this one is finished
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T* bias = (const T*)a.e.bias;
+        const T* res = (const T*)a.e.residual;
+        T4 bq[QUADS], rq[2][QUADS];
+        if (bias) {
+#pragma unroll
+            for (int n = 0; n < QUADS; ++n) bq[n] = *(const T4*)(bias + min(column(n), a.np - 4));
+        }
+        auto fetch = [&](int j) __attribute__((always_inline)) {
+            const int q = min(q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1)), a.nq - 1);
+            const T* row = res + (size_t)q * a.e.ldr;
+#pragma unroll
+            for (int n = 0; n < QUADS; ++n) rq[j & 1][n] = *(const T4*)(row + min(column(n), a.np - 4));
+        };
+        if (res) fetch(0);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            if (res && j + 1 < NQ) fetch(j + 1);
+            const int q = q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1));
+#pragma unroll
+            for (int n = 0; n < QUADS; ++n) {
+                const f32x4 v = quad(n, j);
+                const int p = column(n);
+                float z[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = bias ? a.e.alpha * v[i] + to_f32(bq[n][i]) : a.e.alpha * v[i];
+                const bool store = q < a.nq && p < a.np;
+                const size_t at = (size_t)q * a.e.ldo + p;
+                if (a.e.pre && store) {
+                    T4 t;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[i] = round_pre<T>(z[i]);
+                    *(T4*)((T*)a.e.pre + at) = t;
+                }
+                T4 t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y = activate<T>(z[i], a.e.act);
+                    if (res) y += a.e.beta * to_f32(rq[j & 1][n][i]);
+                    t[i] = from_f32<T>(y);
+                }
+                if (store) *(T4*)((T*)a.e.out + at) = t;
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         const int q = q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1));
         if (q >= a.nq) continue;
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int b = 0; b < M::QUADS; ++b) {
-                const int p = p0 + wp * TP + i * M::FR + b * 8 + 4 * g;
-                if (p >= a.np) continue;
-                const float v[4] = {acc[i][j][4 * b], acc[i][j][4 * b + 1], acc[i][j][4 * b + 2], acc[i][j][4 * b + 3]};
-                if (a.splits > 1)
-                    *(f32x4*)(a.partial + ((size_t)split * a.nq + q) * a.np4 + p) = (f32x4){v[0], v[1], v[2], v[3]};
-                else
-                    epilogue4<T>(a.e, v, q, p, a.np);
-            }
+        for (int n = 0; n < QUADS; ++n) {
+            const int p = column(n);
+            if (p >= a.np) continue;
+            const f32x4 t = quad(n, j);
+            const float v[4] = {t[0], t[1], t[2], t[3]};
+            if (a.splits > 1) *(f32x4*)(a.partial + ((size_t)split * a.nq + q) * a.np4 + p) = t;
+            else epilogue4<T>(a.e, v, q, p, a.np);
+        }
     }
 }
 
@@ -341,7 +455,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long ldg, const
         for (int i = 0; i < 4; ++i) {
             if (c + i < n) {
                 const float g = to_f32(dy[r * ldg + c + i]);
-                const float d = act == ACT_NONE ? g : g * activate_slope(to_f32(pre[r * ldpre + c + i]), act);
+                const float d = act == ACT_NONE ? g : g * activate_slope<T>(to_f32(pre[r * ldpre + c + i]), act);
                 sum[i] += d;
                 if (dz) dz[r * (long)ldz + c + i] = from_f32<T>(d);
                 if (dr) dr[r * (long)n + c + i] = from_f32<T>(beta * g);
@@ -387,17 +501,17 @@ static bool ready(const void* p, int64_t ld, int64_t cols, int es) {
     return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && (cols * es) % 16 == 0;
 }
 
-// Splits of k for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least
-// four steps of k.
+// Tiles of 256 x 256 (16-bit types, eight waves) where there are enough of them for every compute unit, else of 128 x 128 (four waves).  Splits of k
+// for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least four steps of k.
 struct Shape { int big, tiles_p, tiles_q, splits, k_split; };
 static Shape shape_of(int64_t np, int64_t nq, int64_t nk, int dtype) {
     Shape s;
     const int step = 128 / elem_size(dtype);
-    s.big = 128;
+    s.big = dtype != NEMO_F32 && np > 192 && nq > 192 && ((np + 255) / 256) * ((nq + 255) / 256) >= 240 ? 256 : 128;
     s.tiles_p = (int)((np + s.big - 1) / s.big);
     s.tiles_q = (int)((nq + s.big - 1) / s.big);
     const int64_t tiles = (int64_t)s.tiles_p * s.tiles_q, steps = (nk + step - 1) / step;
-    int64_t want = tiles >= 256 ? 1 : 512 / tiles;
+    int64_t want = tiles >= 256 || s.big == 256 ? 1 : 512 / tiles;
     if (want > steps / 4) want = steps / 4;
     if (want < 1) want = 1;
     const int64_t per = steps > 0 ? (steps + want - 1) / want : 1;
@@ -412,7 +526,11 @@ static size_t partial_bytes(int64_t np, int64_t nq, const Shape& s) {
 template <typename T, bool PT, bool QT>
 static void launch_gemm_typed(const GemmArgs& a, hipStream_t st) {
     const long wgs = (long)a.tiles_p * a.tiles_q * a.splits;
-    hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    if (a.big == 256) {
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, PT, QT>), dim3((unsigned)wgs), dim3(512), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    }
     if (a.splits > 1) {
         const long threads = (long)(a.np4 / 4) * a.nq;
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
@@ -457,7 +575,7 @@ static GemmArgs gemm_args(Operand P, Operand Q, int64_t np, int64_t nq, int64_t 
     GemmArgs a = {};
     a.P = P.p; a.Q = Q.p; a.ldp = P.ld; a.ldq = Q.ld;
     a.np = (int)np; a.nq = (int)nq; a.nk = (int)nk;
-    a.tiles_p = s.tiles_p; a.tiles_q = s.tiles_q; a.splits = s.splits; a.k_split = s.k_split;
+    a.big = s.big; a.tiles_p = s.tiles_p; a.tiles_q = s.tiles_q; a.splits = s.splits; a.k_split = s.k_split;
     a.partial = (float*)partial;
     a.np4 = (int)((np + 3) / 4 * 4);
     a.e.alpha = 1.0f;
@@ -482,6 +600,13 @@ static int check_linear(const char* who, int64_t M, int64_t N, int64_t K, int dt
     return NEMO_OK;
 }
 
+// Offsets within a tile of 256 rows are 32-bit.  cols: the contiguous extent, what a packed copy has.
+static int check_stride(const char* who, const void* p, int64_t ld, int64_t cols, int dtype) {
+    const int es = elem_size(dtype);
+    if ((ready(p, ld, cols, es) ? ld : pad16(cols, es)) * es > (1 << 22)) return fail(NEMO_ERR_UNSUPPORTED, "%s: rows more than 4 MiB apart", who);
+    return NEMO_OK;
+}
+
 }  // namespace nemo
 
 using namespace nemo;
@@ -501,6 +626,7 @@ extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64
     if (M == 0 || N == 0) return NEMO_OK;
     if (!y || (K > 0 && (!x || !weight))) return fail(NEMO_ERR_INVALID, "nemo_linear: null argument");
     if ((K > 0 && (ldx < K || ldw < K)) || (residual && ldr < N)) return fail(NEMO_ERR_INVALID, "nemo_linear: a row stride shorter than the row");
+    if (K > 0 && ((rc = check_stride("nemo_linear", x, ldx, K, dtype)) || (rc = check_stride("nemo_linear", weight, ldw, K, dtype)))) return rc;
     const size_t need = nemo_linear_workspace(x, ldx, weight, ldw, M, N, K, dtype);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -567,6 +693,11 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
     if (activation != ACT_NONE && M > 0 && N > 0 && !pre) return fail(NEMO_ERR_INVALID, "nemo_linear_backward: the activation needs `pre`");
     if (M > 0 && N > 0 && K > 0 && ((grad_x && (!weight || ldw < K)) || (grad_weight && (!x || ldx < K))))
         return fail(NEMO_ERR_INVALID, "nemo_linear_backward: null operand or a row stride shorter than the row");
+    if (M > 0 && N > 0 && K > 0 && (grad_x || grad_weight)) {
+        if ((rc = check_stride("nemo_linear_backward", grad_y, ldg, N, dtype)) || (grad_x && (rc = check_stride("nemo_linear_backward", weight, ldw, K, dtype))) ||
+            (grad_weight && (rc = check_stride("nemo_linear_backward", x, ldx, K, dtype))))
+            return rc;
+    }
     const size_t need = nemo_linear_backward_workspace(grad_y, ldg, x, ldx, weight, ldw, M, N, K, dtype, activation);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
