@@ -31,6 +31,14 @@ template <typename T> __device__ inline T from_f32(float x) { return (T)x; }    
 
 __device__ inline float neg_inf() { return -__builtin_inff(); }
 
+// N elements at any element's address: 8- and 16-byte accesses need no alignment on this hardware.
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    typedef T V __attribute__((ext_vector_type(N)));
+    V v;
+};
+template <int N, typename T> __device__ inline typename Loose<T, N>::V load_loose(const T* p) { return ((const Loose<T, N>*)p)->v; }
+template <int N, typename T> __device__ inline void store_loose(T* p, typename Loose<T, N>::V v) { ((Loose<T, N>*)p)->v = v; }
+
 // ---- matrix cores ---------------------------------------------------------------------------------------------------------------
 template <typename T> struct Mma;
 

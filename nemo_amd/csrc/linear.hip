@@ -3,7 +3,7 @@
 // One tiled product serves the forward pass and both weight- and input-gradients.  It computes
 //     C[q][p] = sum_k P(p, k) Q(q, k)
 // where p, the column of the result that is contiguous in memory, is the FIRST operand of the matrix instruction, so that a lane ends
-// up with four consecutive columns of one row and stores them with one instruction.  An operand is "plain" when k is contiguous in
+// up with four consecutive columns of one row.  An operand is "plain" when k is contiguous in
 // memory and "transposed" when its row index is:
 //     y  = x W^T       p = output channel (W plain),  q = row of x (plain),          k = input channel
 //     dx = dz W        p = input channel (W transposed), q = row of dz (plain),      k = output channel
@@ -77,7 +77,6 @@ struct Epilogue {
     void* out;                 // [nq][ldo]
     long ldo;
     void* pre;                 // [nq][ldo]: alpha acc + bias, or null
-    int vec;                   // rows of out, pre and residual start on four elements, and so does their end
 };
 
 struct GemmArgs {
@@ -100,68 +99,38 @@ template <> __device__ inline f16 round_pre<f16>(float z) {
     return h;
 }
 
-// Four consecutive columns p .. p + 3 of row q.
-template <typename T>
-__device__ inline void epilogue4(const Epilogue& e, const float v[4], int q, int p, int np) {
-    const int n = np - p < 4 ? np - p : 4;
-    const T* bias = (const T*)e.bias;
-    const T* res = e.residual ? (const T*)e.residual + (size_t)q * e.ldr + p : nullptr;
-    T* out = (T*)e.out + (size_t)q * e.ldo + p;
-    T* pre = e.pre ? (T*)e.pre + (size_t)q * e.ldo + p : nullptr;
-    float z[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (e.vec) {
-        if (bias) {
-            const T4 b = *(const T4*)(bias + p);
+template <typename T, int N> __device__ inline void activate_all(float (&v)[N], int act) {
+    if (act == ACT_NONE) return;
+    if (act == ACT_RELU) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = e.alpha * v[i] + to_f32(b[i]);
-        } else {
+        for (int i = 0; i < N; ++i) v[i] = activate<T>(v[i], ACT_RELU);
+    } else if (act == ACT_GELU) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = e.alpha * v[i];
-        }
-        if (res) {
-            const T4 t = *(const T4*)res;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = to_f32(t[i]);
-        }
+        for (int i = 0; i < N; ++i) v[i] = activate<T>(v[i], ACT_GELU);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            z[i] = e.alpha * v[i];
-            if (bias && i < n) z[i] += to_f32(bias[p + i]);
-            if (res && i < n) r[i] = to_f32(res[i]);
+        for (int i = 0; i < N; ++i) v[i] = activate<T>(v[i], ACT_SILU);
+    }
+}
+
+// Up to N consecutive columns from p on of row q, those below np.
+template <typename T, int N>
+__device__ inline void epilogue_tail(const Epilogue& e, const float (&acc)[N], int q, int p, int np) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = p + i < np && e.bias ? e.alpha * acc[i] + to_f32(((const T*)e.bias)[p + i]) : e.alpha * acc[i];
+    if (e.pre) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (p + i < np) ((T*)e.pre)[(size_t)q * e.ldo + p + i] = round_pre<T>(v[i]);
+    }
+    activate_all<T, N>(v, e.act);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (p + i < np) {
+            const float r = e.residual ? v[i] + e.beta * to_f32(((const T*)e.residual)[(size_t)q * e.ldr + p + i]) : v[i];
+            ((T*)e.out)[(size_t)q * e.ldo + p + i] = from_f32<T>(r);
         }
-    }
-    if (pre) {
-        if (e.vec) {
-            T4 t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = round_pre<T>(z[i]);
-            *(T4*)pre = t;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < n) pre[i] = round_pre<T>(z[i]);
-        }
-    }
-    if (e.act != ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = activate<T>(z[i], e.act);
-    }
-    if (res) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] += e.beta * r[i];
-    }
-    if (e.vec) {
-        T4 t;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(z[i]);
-        *(T4*)out = t;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) out[i] = from_f32<T>(z[i]);
-    }
 }
 
 // Exclusive-or of the 16-byte chunk index of k row `k` in a transposed 16-bit tile: the 16 rows that one fragment read touches (8 g + 0..3
@@ -321,8 +290,8 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
             multiply(1, next, 0);                                      // behind the last tile what is read is of no use, and none is made of it
         };
         load_any(lds0, 0);
-        load_any(lds1, 1);
         __syncthreads();
+        load_any(lds1, 1);
 #pragma unroll
         for (int n = 0; n < HALF * (NP + NQ); ++n) read(lds0, 0, n);
         int t = 0;
@@ -336,74 +305,78 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
         }
     }
 
-    const int g = lane / M::FR;
-    constexpr int QUADS = NP * M::QUADS;                                // quads of columns of a lane
-    auto column = [&](int n) __attribute__((always_inline)) { return p0 + wp * TP + n / M::QUADS * M::FR + n % M::QUADS * 8 + 4 * g; };
-    auto quad = [&](int n, int j) __attribute__((always_inline)) {
-        const typename M::Acc& c = acc[n / M::QUADS][j];
-        const int b = n % M::QUADS;
-        return (f32x4){c[4 * b], c[4 * b + 1], c[4 * b + 2], c[4 * b + 3]};
-    };
-    if (a.splits == 1 && a.e.vec) {
-        // bias once, a row's residual all at once, the next row's while this one is finished
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const T* bias = (const T*)a.e.bias;
-        const T* res = (const T*)a.e.residual;
-        T4 bq[QUADS], rq[2][QUADS];
-        if (bias) {
+    // Through LDS into rows: a wave writes its results there (f32, in the buffers that held the tiles) and takes them back E consecutive columns
+    // a lane, so that a row goes to memory in one piece, whatever its start, and the code that finishes a value stands here once.  Chunk c
+    // (16 bytes) of row r lies at c ^ (r & 15).
+    constexpr int E = 16 / (int)sizeof(T), REGION = (BP + BQ) * 256 / WAVES, ROWS = REGION / (TP * 4), PASSES = TQ / ROWS > 0 ? TQ / ROWS : 1;
+    constexpr int FRAGS = NQ / PASSES, LANES = TP / E, ITERS = FRAGS * M::FR * LANES / 64, BATCH = 4;
+    static_assert(FRAGS * M::FR * TP * 4 <= REGION && TP / 4 >= 16 && ITERS % BATCH == 0, "a pass fits the wave's share of LDS");
+    char* region = (wave < WAVES / 2 ? lds0 : lds1) + wave % (WAVES / 2) * REGION;
+    const T* bias = (const T*)a.e.bias;
+    const T* res = (const T*)a.e.residual;
+    const int c0 = lane % LANES * E, p = p0 + wp * TP + c0, whole = p + E <= a.np;
+    typename Loose<T, E>::V bv = {};
+    if (bias && whole) bv = load_loose<E>(bias + p);
 #pragma unroll
-            for (int n = 0; n < QUADS; ++n) bq[n] = *(const T4*)(bias + min(column(n), a.np - 4));
-        }
-        auto fetch = [&](int j) __attribute__((always_inline)) {
-            const int q = min(q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1)), a.nq - 1);
-            const T* row = res + (size_t)q * a.e.ldr;
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncthreads();                                               // nobody reads the tiles, or the pass before, any more
 #pragma unroll
-            for (int n = 0; n < QUADS; ++n) rq[j & 1][n] = *(const T4*)(row + min(column(n), a.np - 4));
-        };
-        if (res) fetch(0);
+        for (int j = 0; j < FRAGS; ++j)
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-            if (res && j + 1 < NQ) fetch(j + 1);
-            const int q = q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1));
+            for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int n = 0; n < QUADS; ++n) {
-                const f32x4 v = quad(n, j);
-                const int p = column(n);
-                float z[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = bias ? a.e.alpha * v[i] + to_f32(bq[n][i]) : a.e.alpha * v[i];
-                const bool store = q < a.nq && p < a.np;
-                const size_t at = (size_t)q * a.e.ldo + p;
-                if (a.e.pre && store) {
-                    T4 t;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] = round_pre<T>(z[i]);
-                    *(T4*)((T*)a.e.pre + at) = t;
+                for (int b = 0; b < M::QUADS; ++b) {
+                    const typename M::Acc& v = acc[i][pass * FRAGS + j];
+                    const int r = j * M::FR + (lane & (M::FR - 1)), c = (i * M::FR + b * 8 + 4 * (lane / M::FR)) / 4;
+                    *(f32x4*)(region + r * (TP * 4) + ((c ^ (r & 15)) << 4)) = (f32x4){v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
                 }
-                T4 t;
+        __syncthreads();
+#pragma unroll 1
+        for (int it = 0; it < ITERS; it += BATCH) {
+            typename Loose<T, E>::V rv[BATCH] = {};
+            if (res && whole) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float y = activate<T>(z[i], a.e.act);
-                    if (res) y += a.e.beta * to_f32(rq[j & 1][n][i]);
-                    t[i] = from_f32<T>(y);
+                for (int n = 0; n < BATCH; ++n) {
+                    const int q = min(q0 + wq * TQ + pass * FRAGS * M::FR + ((it + n) * 64 + lane) / LANES, a.nq - 1);
+                    rv[n] = load_loose<E>(res + (size_t)q * a.e.ldr + p);
                 }
-                if (store) *(T4*)((T*)a.e.out + at) = t;
             }
-        }
-        return;
-    }
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-        const int q = q0 + wq * TQ + j * M::FR + (lane & (M::FR - 1));
-        if (q >= a.nq) continue;
+            for (int n = 0; n < BATCH; ++n) {
+                const int r = ((it + n) * 64 + lane) / LANES, q = q0 + wq * TQ + pass * FRAGS * M::FR + r;
+                float v[E];
 #pragma unroll
-        for (int n = 0; n < QUADS; ++n) {
-            const int p = column(n);
-            if (p >= a.np) continue;
-            const f32x4 t = quad(n, j);
-            const float v[4] = {t[0], t[1], t[2], t[3]};
-            if (a.splits > 1) *(f32x4*)(a.partial + ((size_t)split * a.nq + q) * a.np4 + p) = t;
-            else epilogue4<T>(a.e, v, q, p, a.np);
+                for (int k = 0; k < E / 4; ++k) {
+                    const f32x4 t = *(const f32x4*)(region + r * (TP * 4) + (((c0 / 4 + k) ^ (r & 15)) << 4));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[4 * k + i] = t[i];
+                }
+                if (q >= a.nq || p >= a.np) continue;
+                if (a.splits > 1) {
+#pragma unroll
+                    for (int k = 0; k < E / 4; ++k)
+                        if (p + 4 * k < a.np)
+                            *(f32x4*)(a.partial + ((size_t)split * a.nq + q) * a.np4 + p + 4 * k) = (f32x4){v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                    continue;
+                }
+                if (!whole) {
+                    epilogue_tail<T>(a.e, v, q, p, a.np);
+                    continue;
+                }
+                const size_t at = (size_t)q * a.e.ldo + p;
+                typename Loose<T, E>::V t;
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i] = a.e.alpha * v[i] + to_f32(bv[i]);
+                if (a.e.pre) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) t[i] = round_pre<T>(v[i]);
+                    store_loose<E>((T*)a.e.pre + at, t);
+                }
+                activate_all<T, E>(v, a.e.act);
+#pragma unroll
+                for (int i = 0; i < E; ++i) t[i] = from_f32<T>(res ? v[i] + a.e.beta * to_f32(rv[n][i]) : v[i]);
+                store_loose<E>((T*)a.e.out + at, t);
+            }
         }
     }
 }
@@ -421,58 +394,89 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += t[i];
     }
-    epilogue4<T>(a.e, v, q, p, a.np);
+    epilogue_tail<T>(a.e, v, q, p, a.np);
 }
 
-// rows x cols (row stride ld) -> rows x ld_out, the columns beyond cols zero; 32-bit words of the copy a thread, ld_out a multiple of 16 bytes.
+// rows x cols (row stride ld, any start) -> rows x ld_out on 16 bytes, the columns beyond cols zero; 16 bytes of the copy a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* src, long ld, long rows, int cols, T* dst, int ld_out) {
     constexpr int E = 16 / (int)sizeof(T);
-    const int per_row = ld_out / E;
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= rows * per_row) return;
-    const long r = id / per_row;
-    const int c = (int)(id % per_row) * E;
-    const T* s = src + r * ld + c;
-    union { T t[E]; u32x4 v; } u;
+    const uint32_t per_row = ld_out / E;
+    const uint32_t id = blockIdx.x * 256u + threadIdx.x;                // fewer than 2^32 threads: see check_linear
+    const uint32_t r = id / per_row;
+    if (r >= rows) return;
+    const int c = (int)(id - r * per_row) * E;
+    const T* s = src + (long)r * ld + c;
+    typename Loose<T, E>::V v = {};
+    if (c + E <= cols) {
+        v = load_loose<E>(s);
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) u.t[i] = c + i < cols ? s[i] : (T)0.0f;
-    *(u32x4*)(dst + r * (long)ld_out + c) = u.v;
+        for (int i = 0; i < E; ++i)
+            if (c + i < cols) v[i] = s[i];
+    }
+    *(typename Loose<T, E>::V*)(dst + (long)r * ld_out + c) = v;
 }
 
 // dz = dy act'(pre) (rounded to T because the matrix cores take T), dr = beta dy, and per block of rows the column sums of the unrounded
-// dz (for the bias).  A workgroup takes 64 columns x ROWS rows: 16 threads of four columns, 16 rows at a time.
-constexpr int kSlopeRows = 256;
+// dz (for the bias).  A workgroup takes 256 columns x ROWS rows: 32 threads of eight columns, eight rows at a time.  Bound by memory; rows
+// may start at any element.
+constexpr int kSlopeRows = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long ldg, const T* pre, long ldpre, long m, int n, int act, float beta,
                                                     T* dz, int ldz, T* dr, float* col_partial, int np4) {
-    const int c = blockIdx.x * 64 + (threadIdx.x & 15) * 4, ry = threadIdx.x >> 4;
+    typedef typename Loose<T, 8>::V T8;
+    const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8, ry = threadIdx.x >> 5;
     const long r0 = (long)blockIdx.y * kSlopeRows;
     const long r1 = r0 + kSlopeRows < m ? r0 + kSlopeRows : m;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (long r = r0 + ry; r < r1; r += 16) {
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (c + 8 <= n) {
+#pragma unroll 4
+        for (long r = r0 + ry; r < r1; r += 8) {
+            const T8 g = load_loose<8>(dy + r * ldg + c);
+            T8 p = {}, d;
+            if (act != ACT_NONE) p = load_loose<8>(pre + r * ldpre + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (c + i < n) {
-                const float g = to_f32(dy[r * ldg + c + i]);
-                const float d = act == ACT_NONE ? g : g * activate_slope<T>(to_f32(pre[r * ldpre + c + i]), act);
-                sum[i] += d;
-                if (dz) dz[r * (long)ldz + c + i] = from_f32<T>(d);
-                if (dr) dr[r * (long)n + c + i] = from_f32<T>(beta * g);
-            } else if (dz && c + i < ldz) {
-                dz[r * (long)ldz + c + i] = (T)0.0f;
+            for (int i = 0; i < 8; ++i) {
+                const float x = act == ACT_NONE ? to_f32(g[i]) : to_f32(g[i]) * activate_slope<T>(to_f32(p[i]), act);
+                sum[i] += x;
+                d[i] = from_f32<T>(x);
+            }
+            if (dz) store_loose<8>(dz + r * (long)ldz + c, d);
+            if (dr) {
+                T8 t;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(beta * to_f32(g[i]));
+                store_loose<8>(dr + r * (long)n + c, t);
+            }
+        }
+    } else if (c < (dz ? ldz : n)) {
+        for (long r = r0 + ry; r < r1; r += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (c + i < n) {
+                    const float g = to_f32(dy[r * ldg + c + i]);
+                    const float x = act == ACT_NONE ? g : g * activate_slope<T>(to_f32(pre[r * ldpre + c + i]), act);
+                    sum[i] += x;
+                    if (dz) dz[r * (long)ldz + c + i] = from_f32<T>(x);
+                    if (dr) dr[r * (long)n + c + i] = from_f32<T>(beta * g);
+                } else if (dz && c + i < ldz) {
+                    dz[r * (long)ldz + c + i] = (T)0.0f;
+                }
             }
         }
     }
     if (!col_partial) return;
-    __shared__ float s[16][64];
+    __shared__ float s[8][256 + 8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[ry][(threadIdx.x & 15) * 4 + i] = sum[i];
+    for (int i = 0; i < 8; ++i) s[ry][(threadIdx.x & 31) * 8 + i] = sum[i];
     __syncthreads();
-    if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < np4) {
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col < np4) {
         float t = 0.0f;
-        for (int i = 0; i < 16; ++i) t += s[i][threadIdx.x];
-        col_partial[(size_t)blockIdx.y * np4 + blockIdx.x * 64 + threadIdx.x] = t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x];
+        col_partial[(size_t)blockIdx.y * np4 + col] = t;
     }
 }
 
@@ -501,13 +505,15 @@ static bool ready(const void* p, int64_t ld, int64_t cols, int es) {
     return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && (cols * es) % 16 == 0;
 }
 
-// Tiles of 256 x 256 (16-bit types, eight waves) where there are enough of them for every compute unit, else of 128 x 128 (four waves).  Splits of k
+// Tiles of 256 x 256 (16-bit types, both operands plain, eight waves) where there are enough of them for every compute unit, else of 128 x 128 (four
+// waves).  8192 x 4096 x 4096 bf16: 218 us against 315 (128 x 128).  The addresses of transposed fragments take too many registers for the
+// large tile (460 us, against 313 with the small one).  Splits of k
 // for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least four steps of k.
 struct Shape { int big, tiles_p, tiles_q, splits, k_split; };
-static Shape shape_of(int64_t np, int64_t nq, int64_t nk, int dtype) {
+static Shape shape_of(int64_t np, int64_t nq, int64_t nk, int dtype, bool transposed) {
     Shape s;
     const int step = 128 / elem_size(dtype);
-    s.big = dtype != NEMO_F32 && np > 192 && nq > 192 && ((np + 255) / 256) * ((nq + 255) / 256) >= 240 ? 256 : 128;
+    s.big = dtype != NEMO_F32 && !transposed && np > 192 && nq > 192 && ((np + 255) / 256) * ((nq + 255) / 256) >= 240 ? 256 : 128;
     s.tiles_p = (int)((np + s.big - 1) / s.big);
     s.tiles_q = (int)((nq + s.big - 1) / s.big);
     const int64_t tiles = (int64_t)s.tiles_p * s.tiles_q, steps = (nk + step - 1) / step;
@@ -527,7 +533,7 @@ template <typename T, bool PT, bool QT>
 static void launch_gemm_typed(const GemmArgs& a, hipStream_t st) {
     const long wgs = (long)a.tiles_p * a.tiles_q * a.splits;
     if (a.big == 256) {
-        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, PT, QT>), dim3((unsigned)wgs), dim3(512), 0, st, a);
+        if constexpr (sizeof(T) == 2 && !PT) hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, PT, QT>), dim3((unsigned)wgs), dim3(512), 0, st, a);
     } else {
         hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
     }
@@ -615,7 +621,7 @@ extern "C" size_t nemo_linear_workspace(const void* x, int64_t ldx, const void* 
                                         int32_t dtype) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     const int es = elem_size(dtype);
-    return operand_bytes(x, ldx, M, K, es) + operand_bytes(weight, ldw, N, K, es) + partial_bytes(N, M, shape_of(N, M, K, dtype));
+    return operand_bytes(x, ldx, M, K, es) + operand_bytes(weight, ldw, N, K, es) + partial_bytes(N, M, shape_of(N, M, K, dtype, false));
 }
 
 extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
@@ -638,11 +644,9 @@ extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64
         P = operand(dtype, weight, ldw, N, K, ws, st);
         Q = operand(dtype, x, ldx, M, K, ws, st);
     }
-    const Shape s = shape_of(N, M, K, dtype);
+    const Shape s = shape_of(N, M, K, dtype, false);
     GemmArgs a = gemm_args(P, Q, N, M, K, s, ws);
-    a.e = {alpha, beta, activation, bias, residual, ldr, y, N, pre, 0};
-    a.e.vec = N % 4 == 0 && ((uintptr_t)y & (4 * es - 1)) == 0 && (!pre || ((uintptr_t)pre & (4 * es - 1)) == 0) &&
-              (!bias || ((uintptr_t)bias & (4 * es - 1)) == 0) && (!residual || (((uintptr_t)residual & (4 * es - 1)) == 0 && ldr % 4 == 0));
+    a.e = {alpha, beta, activation, bias, residual, ldr, y, N, pre};
     launch_gemm(dtype, a, false, false, st);
     HIP_TRY(hipGetLastError());
     return NEMO_OK;
@@ -658,7 +662,7 @@ extern "C" size_t nemo_linear_backward_workspace(const void* grad_y, int64_t ldg
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return column_bytes(M, N);
     const int es = elem_size(dtype);
-    const size_t dx = partial_bytes(K, M, shape_of(K, M, N, dtype)), dw = partial_bytes(K, N, shape_of(K, N, M, dtype));
+    const size_t dx = partial_bytes(K, M, shape_of(K, M, N, dtype, true)), dw = partial_bytes(K, N, shape_of(K, N, M, dtype, true));
     return (slope_needed(grad_y, ldg, N, dtype, activation) ? packed_bytes(M, N, es) : 0) + operand_bytes(x, ldx, M, K, es) +
            operand_bytes(weight, ldw, N, K, es) + (dx > dw ? dx : dw) + column_bytes(M, N);
 }
@@ -672,7 +676,7 @@ static void launch_slope(const void* dy, int64_t ldg, const void* pre, int64_t M
     const int64_t blocks = (M + kSlopeRows - 1) / kSlopeRows;
     for (int64_t b0 = 0; b0 < blocks; b0 += 65535) {
         const int64_t nb = blocks - b0 < 65535 ? blocks - b0 : 65535, r0 = b0 * kSlopeRows;
-        hipLaunchKernelGGL((slope_kernel<T>), dim3((width + 63) / 64, (unsigned)nb), dim3(256), 0, st, (const T*)dy + r0 * ldg, (long)ldg,
+        hipLaunchKernelGGL((slope_kernel<T>), dim3((width + 255) / 256, (unsigned)nb), dim3(256), 0, st, (const T*)dy + r0 * ldg, (long)ldg,
                            pre ? (const T*)pre + r0 * N : (const T*)nullptr, (long)N, (long)(M - r0), (int)N, act, beta,
                            dz ? (T*)dz + r0 * ldz : (T*)nullptr, ldz, dr ? (T*)dr + r0 * N : (T*)nullptr,
                            partial ? partial + (size_t)b0 * np4 : (float*)nullptr, np4);
@@ -728,19 +732,17 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
     }
     if (grad_x && M > 0 && K > 0) {
         Operand W = N > 0 ? operand(dtype, weight, ldw, N, K, ws, st) : Operand{weight, ldw};
-        const Shape s = shape_of(K, M, N, dtype);
+        const Shape s = shape_of(K, M, N, dtype, true);
         GemmArgs a = gemm_args(W, dz, K, M, N, s, ws);
-        a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_x, K, nullptr, 0};
-        a.e.vec = K % 4 == 0 && ((uintptr_t)grad_x & (4 * es - 1)) == 0;
-        launch_gemm(dtype, a, true, false, st);
+        a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_x, K, nullptr};
+            launch_gemm(dtype, a, true, false, st);
     }
     if (grad_weight && N > 0 && K > 0) {
         Operand X = M > 0 ? operand(dtype, x, ldx, M, K, ws, st) : Operand{x, ldx};
-        const Shape s = shape_of(K, N, M, dtype);
+        const Shape s = shape_of(K, N, M, dtype, true);
         GemmArgs a = gemm_args(X, dz, K, N, M, s, ws);
-        a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_weight, K, nullptr, 0};
-        a.e.vec = K % 4 == 0 && ((uintptr_t)grad_weight & (4 * es - 1)) == 0;
-        launch_gemm(dtype, a, true, true, st);
+        a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_weight, K, nullptr};
+            launch_gemm(dtype, a, true, true, st);
     }
     HIP_TRY(hipGetLastError());
     return NEMO_OK;
