@@ -26,25 +26,24 @@ __device__ inline void insert(float (&tv)[TOP], int (&tp)[TOP], float z, int pla
     tv[0] = fmaxf(z, tv[0]);
 }
 
-// GENERAL: with weights, with a list (its order is that of the scores), or with hardly any scale; see softmax_state.h for the two forms of the state.  The sign of the scale goes into the
-// owners' fragments where the state is kept of the products.
+// NP: pieces of a value (bank_tiles.h).  GENERAL: with weights, with a list (its order is that of the scores), or with hardly any scale; see
+// softmax_state.h for the two forms of the state.  The sign of the scale goes into the owners' fragments where the state is kept of the products.
 //
 // Tiles of 32 bank rows; in step n the wave multiplies tile n + 1 while it takes the products of tile n into the state, so that matrix cores
 // and vector units work side by side.  Two tiles in LDS (n + 1, and n + 2 on its way), one barrier a step.
-template <typename T, int CP, int TOP, bool GENERAL>
-__global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forward_kernel(BankArgs a) {
-    typedef Tile<T, CP> L;
-    constexpr int NT = TOP > 0 ? TOP : 1, NKF = CP / Wide<T>::KF;
-    constexpr bool F32 = sizeof(T) == 4;
-    __shared__ __attribute__((aligned(16))) char lds0[L::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds1[L::BYTES];
+template <int NP, int CP, int TOP, bool GENERAL>
+__global__ __launch_bounds__(256, NP * CP > 512 ? 1 : 2) void bank_forward_kernel(BankArgs a) {
+    typedef Tile<CP> L;
+    constexpr int NT = TOP > 0 ? TOP : 1, NKF = CP / kFragK;
+    __shared__ __attribute__((aligned(16))) char lds0[NP * L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[NP * L::BYTES];
     __shared__ int s_again;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int part = (int)(blockIdx.x % a.parts);
     const int own0 = (int)(blockIdx.x / a.parts) * 128 + wave * 32, row = own0 + (lane & 31);
     const bool live = row < a.n_own;
-    u32x4 q[NKF];
-    own_fragments<T, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
+    u32x4 q[NP][NKF];
+    own_fragments<NP, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
     const float* w = a.weights ? a.weights + (live ? row : 0) * a.ldw : nullptr;
     const long long tl = live ? a.targets[row] : -1;
     const int target = tl >= 0 && tl < a.n_other ? (int)tl : -1;
@@ -95,7 +94,7 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
     };
     const int tiles = (a.n_other + 31) / 32;
     const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
-    const Stager<T, CP> stager((const T*)a.other, a.ld_other, a.n_other, a.channels, wave, lane);
+    const Stager<NP, CP> stager(a, wave, lane);
     auto stage = [&](char* lds, int tile) __attribute__((always_inline)) { stager.copy(lds, tile); };
     auto start = [&]() __attribute__((always_inline)) {
         st = empty_state();
@@ -110,7 +109,7 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
             float wv[16], v[16];
             load_weights(wv, t);
             __syncthreads();
-            const f32x16_t pr = products<T, CP>(lds0, q, lane);
+            const f32x16_t pr = products<NP, CP>(lds0, q, lane);
             const int left = a.n_other - t * 32 - 4 * g;               // registers whose row 8 b + i is at least this are beyond the end
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = 8 * (i >> 2) + (i & 3) >= left ? neg_inf() : value(pr, wv, i);
@@ -127,7 +126,7 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
     if (t0 < whole) {
         stage(lds0, t0);
         __syncthreads();
-        f32x16_t pr = products<T, CP>(lds0, q, lane);
+        f32x16_t pr = products<NP, CP>(lds0, q, lane);
         stage(lds1, t0 + 1);
         // `next` holds tile t + 1; `after` held tile t, whose products are in pr.  A slice: a fragment is read (two slices ahead of its use),
         // multiplied, and a share of the 18 units of tile t is done: the largest product, the state raised to it, 16 products added.  Weights
@@ -138,18 +137,24 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
             float wv[16], v[16];
             load_weights(wv, t);
             f32x16_t nxt = {};
-            constexpr int UNITS = 18;
+            constexpr int UNITS = 18, FRAGS = NKF * NP, SLICES = NKF * Pairs<NP>::N;
             float peak = 0.0f;
             u32x4 f[3];
-            f[0] = row_fragment<T, CP>(next, 0, lane);
-            f[1] = row_fragment<T, CP>(next, 1, lane);
+            auto read = [&](int n) __attribute__((always_inline)) {
+                if (n < FRAGS) f[n % 3] = row_fragment<CP>(next + n % NP * L::BYTES, n / NP, lane);
+            };
+            read(0);
+            read(1);
 #pragma unroll
-            for (int i = 0; i < NKF; ++i) {
-                if (i + 2 < NKF) f[(i + 2) % 3] = row_fragment<T, CP>(next, i + 2, lane);
-                settle(f[i % 3]);
-                Wide<T>::run(nxt, f[i % 3], q[i]);
-                const int from = GENERAL ? (2 * i < NKF ? 0 : (2 * i - NKF) * UNITS / NKF) : i * UNITS / NKF;
-                const int to = GENERAL ? (2 * i + 2 < NKF ? 0 : (2 * i + 2 - NKF) * UNITS / NKF) : (i + 1) * UNITS / NKF;
+            for (int i = 0; i < SLICES; ++i) {
+                const int kf = i / Pairs<NP>::N, pair = i % Pairs<NP>::N, n = kf * NP + Pairs<NP>::first(pair);
+                if (Pairs<NP>::second(pair) == 0) {
+                    read(n + 2);
+                    settle(f[n % 3]);
+                }
+                wide_mma(nxt, f[n % 3], q[Pairs<NP>::second(pair)][kf]);
+                const int from = GENERAL ? (2 * i < SLICES ? 0 : (2 * i - SLICES) * UNITS / SLICES) : i * UNITS / SLICES;
+                const int to = GENERAL ? (2 * i + 2 < SLICES ? 0 : (2 * i + 2 - SLICES) * UNITS / SLICES) : (i + 1) * UNITS / SLICES;
 #pragma unroll
                 for (int u = from; u < to; ++u) {
                     if (u == 0) {
@@ -206,21 +211,22 @@ __global__ __launch_bounds__(256, CP * sizeof(T) >= 1024 ? 1 : 2) void bank_forw
         }
 }
 
-template <typename T, int CP>
+template <int NP, int CP>
 static void launch(const BankArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.n_own + 127) / 128 * a.parts));
     const int top = a.out.top;
-    if (a.out.k != 0.0f) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, false>), grid, dim3(256), 0, st, a);
-    else if (top == 0) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 0, true>), grid, dim3(256), 0, st, a);
-    else if (top <= 5) hipLaunchKernelGGL((bank_forward_kernel<T, CP, 5, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((bank_forward_kernel<T, CP, 16, true>), grid, dim3(256), 0, st, a);
+    if (a.out.k != 0.0f) hipLaunchKernelGGL((bank_forward_kernel<NP, CP, 0, false>), grid, dim3(256), 0, st, a);
+    else if (top == 0) hipLaunchKernelGGL((bank_forward_kernel<NP, CP, 0, true>), grid, dim3(256), 0, st, a);
+    else if (top <= 5) hipLaunchKernelGGL((bank_forward_kernel<NP, CP, 5, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((bank_forward_kernel<NP, CP, 16, true>), grid, dim3(256), 0, st, a);
 }
 
 template <> void launch_bank_forward<NEMO_ELEMENT>(const BankArgs& a, hipStream_t st) {
+    constexpr int NP = sizeof(NEMO_ELEMENT) == 4 ? 3 : 1;
     switch (padded_channels(a.channels)) {
-        case 64: launch<NEMO_ELEMENT, 64>(a, st); break;
-        case 128: launch<NEMO_ELEMENT, 128>(a, st); break;
-        default: launch<NEMO_ELEMENT, 256>(a, st);
+        case 64: launch<NP, 64>(a, st); break;
+        case 128: launch<NP, 128>(a, st); break;
+        default: launch<NP, 256>(a, st);
     }
 }
 

@@ -18,11 +18,11 @@ namespace nemo {
 
 // dz of one score or product without the target's share.  In bf16 and without weights m holds m + log2 s, one operation less: off by u |lse|
 // (1e-6 at 16), far below the rounding of dz's pieces.  SAFE: log2 p may be -inf.
-template <typename T, bool GENERAL, bool SAFE>
+template <bool F32, bool GENERAL, bool SAFE>
 __device__ inline float pair_gradient(float v, float k, float m, float log2_s, float c, float g2) {
     float lp2;
     if (GENERAL) lp2 = __builtin_fmaf(v - m, kLog2e, -log2_s);
-    else if (sizeof(T) == 4) lp2 = __builtin_fmaf(k, v, -m) - log2_s;
+    else if (F32) lp2 = __builtin_fmaf(k, v, -m) - log2_s;
     else lp2 = __builtin_fmaf(k, v, -m);
     return SAFE ? prob_gradient(lp2, c, g2) : exp2_fast(lp2) * (c - g2 * lp2);
 }
@@ -30,77 +30,64 @@ __device__ inline float pair_gradient(float v, float k, float m, float log2_s, f
 // A value of the second product's first operand; `clean` turns infinities and NaN into 0 (see bank_gradient_kernel).
 __device__ inline float clean_value(float v) { return __builtin_fabsf(v) <= FLT_MAX ? v : 0.0f; }
 
-// First operand of the second product: columns cb .. cb + 31 (cb a multiple of 32) of the tile's rows, in the order in which the first product's
-// registers hold them.  f32: step b takes registers 4 b .. 4 b + 3, rows 8 b + 4 g + i.  bf16: step b takes registers 8 b .. 8 b + 7, rows
-// 16 b + 8 (e / 4) + 4 g + e % 4, two transposing reads of four rows each (lane i of a group of 16 supplies columns 4 (i % 4) .. + 3 of row
-// i / 4 and receives column i of the four rows).
-template <typename T, int CP>
+// First operand of the second product: columns cb .. cb + 31 (cb a multiple of 32) of the tile's rows, one piece, in the order in which the first
+// product's registers hold them: step b takes registers 8 b .. 8 b + 7, rows 16 b + 8 (e / 4) + 4 g + e % 4, two transposing reads of four
+// rows each (lane i of a group of 16 supplies columns 4 (i % 4) .. + 3 of row i / 4 and receives column i of the four rows).
+template <int CP>
 __device__ inline u32x4 column_fragment(const char* lds, int b, int cb, int lane, bool clean) {
-    typedef Tile<T, CP> L;
-    const int g = lane >> 5;
-    if constexpr (sizeof(T) == 4) {
-        u32x4 v;
+    typedef Tile<CP> L;
+    const int g = lane >> 5, i = lane & 15, t = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    union { i16x4 h[2]; u32x4 v; bf16 t[8]; } u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float x = *(const float*)(lds + L::row(8 * b + i) + L::row(4) * g + L::chunk(cb >> 2, (lane & 31) >> 2, L::flip(4 * g + i)) + (lane & 3) * 4);
-            if (clean) x = clean_value(x);
-            v[i] = __builtin_bit_cast(uint32_t, x);
-        }
-        return v;
-    } else {
-        const int i = lane & 15, t = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-        union { i16x4 h[2]; u32x4 v; bf16 t[8]; } u;
+    for (int e = 0; e < 2; ++e)
+        u.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (NEMO_LDS i16x4*)(lds + L::row(16 * b + 8 * e) + L::row(4) * g + L::row(i >> 2) + L::chunk(cb >> 3, t, L::flip(8 * e + 4 * g + (i >> 2))) + (i & 1) * 8));
+    if (clean)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            u.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (NEMO_LDS i16x4*)(lds + L::row(16 * b + 8 * e) + L::row(4) * g + L::row(i >> 2) + L::chunk(cb >> 3, t, L::flip(8 * e + 4 * g + (i >> 2))) + (i & 1) * 8));
-        if (clean)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u.t[e] = (bf16)clean_value((float)u.t[e]);
-        return u.v;
-    }
+        for (int e = 0; e < 8; ++e) u.t[e] = (bf16)clean_value((float)u.t[e]);
+    return u.v;
 }
 
-// 16 dz of a lane as second operands of the second product: f32 as they are; bf16 as two pieces each, filled two values at a time.
-template <typename T> struct Pieces;
-template <> struct Pieces<float> {
-    static constexpr int STEPS = 4, N = 1;
-    u32x4 p[4][1];
-    __device__ inline void pair(int i, float z0, float z1) {
-        p[i >> 1][0][2 * (i & 1)] = __builtin_bit_cast(uint32_t, z0);
-        p[i >> 1][0][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, z1);
-    }
-    __device__ inline void settle_pair(int) {}
-};
-template <> struct Pieces<bf16> {
-    static constexpr int STEPS = 2, N = 2;
-    u32x4 p[2][2];
+// 16 dz of a lane as second operands of the second product, filled two values at a time.  Rows of one piece: dz = hi + lo, 16 bits, both multiplied.
+// Rows of three pieces: dz of three pieces, paired as in the first product.
+template <int NP> struct Pieces {
+    static constexpr int STEPS = 2, N = NP == 1 ? 2 : 3, PAIRS = NP == 1 ? 2 : 6;
+    static __device__ constexpr int first(int u) { return NP == 1 ? 0 : Pairs<3>::first(u); }       // piece of the rows
+    static __device__ constexpr int second(int u) { return NP == 1 ? u : Pairs<3>::second(u); }     // piece of dz
+    u32x4 p[STEPS][N];
     __device__ inline void pair(int i, float z0, float z1) {
         typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        const bf16x2 hi = {(bf16)z0, (bf16)z1};
-        const uint32_t h = __builtin_bit_cast(uint32_t, hi);
-        const float h0 = __builtin_bit_cast(float, h << 16), h1 = __builtin_bit_cast(float, h & 0xFFFF0000u);
-        const bf16x2 lo = {(bf16)(z0 - h0), (bf16)(z1 - h1)};
-        p[i >> 2][0][i & 3] = h;
-        p[i >> 2][1][i & 3] = __builtin_bit_cast(uint32_t, lo);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const bf16x2 hi = {(bf16)z0, (bf16)z1};
+            const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+            p[i >> 2][n][i & 3] = h;
+            z0 -= __builtin_bit_cast(float, h << 16);
+            z1 -= __builtin_bit_cast(float, h & 0xFFFF0000u);
+        }
     }
     __device__ inline void settle_pair(int i) {
-        uint32_t h = p[i >> 2][0][i & 3], l = p[i >> 2][1][i & 3];
-        asm volatile("" : "+v"(h), "+v"(l));
-        p[i >> 2][0][i & 3] = h;
-        p[i >> 2][1][i & 3] = l;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            uint32_t x = p[i >> 2][n][i & 3];
+            asm volatile("" : "+v"(x));
+            p[i >> 2][n][i & 3] = x;
+        }
     }
 };
 
-template <typename T, int CP>
-__device__ inline void second_product(f32x16_t (&acc)[CP / 32], const char* lds, const Pieces<T>& dz, int lane, bool clean) {
+template <int NP, int CP>
+__device__ inline void second_product(f32x16_t (&acc)[CP / 32], const char* lds, const Pieces<NP>& dz, int lane, bool clean) {
+    typedef Pieces<NP> P;
 #pragma unroll
-    for (int b = 0; b < Pieces<T>::STEPS; ++b)
+    for (int b = 0; b < P::STEPS; ++b)
 #pragma unroll
         for (int x = 0; x < CP / 32; ++x) {
-            const u32x4 f = column_fragment<T, CP>(lds, b, x * 32, lane, clean);
+            u32x4 f[NP];
 #pragma unroll
-            for (int n = 0; n < Pieces<T>::N; ++n) Wide<T>::run(acc[x], f, dz.p[b][n]);
+            for (int n = 0; n < NP; ++n) f[n] = column_fragment<CP>(lds + n * Tile<CP>::BYTES, b, x * 32, lane, clean);
+#pragma unroll
+            for (int u = 0; u < P::PAIRS; ++u) wide_mma(acc[x], f[P::first(u)], dz.p[b][P::second(u)]);
         }
 }
 
@@ -118,15 +105,16 @@ __device__ inline void second_product(f32x16_t (&acc)[CP / 32], const char* lds,
 // operand taken as 0 and with log2 p = -inf allowed for.  Where they are not left out the scores themselves, and with them dz, are NaN, and
 // so stays the result.
 template <typename T, int CP, bool OWN_BANK, bool GENERAL>
-__global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(BankArgs a) {
-    typedef Tile<T, CP> L;
+__global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1 : 2) void bank_gradient_kernel(BankArgs a) {
+    typedef Tile<CP> L;
     constexpr bool F32 = sizeof(T) == 4, SPLIT = GENERAL || F32;       // log2 s apart from m
-    constexpr bool SIDE_BY_SIDE = CP <= 128 && !(F32 && GENERAL);
-    constexpr int NX = CP / 32, NKF = CP / Wide<T>::KF;
-    __shared__ __attribute__((aligned(16))) char lds0[L::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds1[L::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds2[SIDE_BY_SIDE ? L::BYTES : 16];
-    __shared__ __attribute__((aligned(16))) char lds3[SIDE_BY_SIDE ? L::BYTES : 16];
+    constexpr bool SIDE_BY_SIDE = CP <= 128;
+    constexpr int NP = F32 ? 3 : 1, NX = CP / 32, NKF = CP / kFragK;
+    typedef Pieces<NP> Dz;
+    __shared__ __attribute__((aligned(16))) char lds0[NP * L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[NP * L::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds2[SIDE_BY_SIDE ? NP * L::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) char lds3[SIDE_BY_SIDE ? NP * L::BYTES : 16];
     __shared__ __attribute__((aligned(16))) float s_coef0[OWN_BANK ? K_COUNT : 1][64];
     __shared__ __attribute__((aligned(16))) float s_coef1[OWN_BANK ? K_COUNT : 1][64];
     __shared__ __attribute__((aligned(16))) float s_coef2[OWN_BANK && SIDE_BY_SIDE ? K_COUNT : 1][64];
@@ -136,8 +124,8 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
     const int part = (int)(blockIdx.x % a.parts);
     const int own0 = (int)(blockIdx.x / a.parts) * 128 + wave * 32, own = own0 + (lane & 31);
     const bool live = own < a.n_own;
-    u32x4 q[NKF];
-    own_fragments<T, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
+    u32x4 q[NP][NKF];
+    own_fragments<NP, CP>(q, a, own0, lane, !GENERAL && a.scale < 0.0f);
     const int n_coef = coef_rows(OWN_BANK ? a.n_other : a.n_own);
     const float k = a.out.k;
     float m = 0.0f, log2_s = 0.0f, c = 0.0f, g2 = 0.0f;               // of an owner beyond the last: dz = 0
@@ -151,7 +139,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
     if (GENERAL && a.weights) w = OWN_BANK ? a.weights + (live ? own : 0) : a.weights + (live ? own : 0) * a.ldw;
     f32x16_t acc[NX];
 
-    const Stager<T, CP> stager((const T*)a.other, a.ld_other, a.n_other, a.channels, wave, lane);
+    const Stager<NP, CP> stager(a, wave, lane);
     auto stage = [&](char* lds, float (*coef)[64], int tile) __attribute__((always_inline)) {
         stager.copy(lds, tile);
         if (OWN_BANK) {
@@ -196,7 +184,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
     auto differentiate = [&](const f32x16_t& pr, const float (&wv)[16], const Quad& k4, int i, int tile, auto safe_tag) __attribute__((always_inline)) {
         constexpr bool SAFE = decltype(safe_tag)::value || GENERAL;
         const float s = !GENERAL ? pr[i] : w ? score(pr[i], a.scale, wv[i]) : score(pr[i], a.scale);
-        const float d = pair_gradient<T, GENERAL, SAFE>(s, k, k4.m[i & 3], k4.s[i & 3], k4.c[i & 3], k4.g2[i & 3]);
+        const float d = pair_gradient<F32, GENERAL, SAFE>(s, k, k4.m[i & 3], k4.s[i & 3], k4.c[i & 3], k4.g2[i & 3]);
         // rows beyond the last are zeros, but where all scores are far below 0 the probability of a 0 is not even finite
         return SAFE && !GENERAL && !OWN_BANK && tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= a.n_other ? 0.0f : d;
     };
@@ -214,10 +202,10 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
             // an owner that is left out for that row
             if (GENERAL && w && tr == own && w[(size_t)(tile * 32 + r) * a.ldw] == __builtin_inff()) z[i] = 0.0f;
         }
-        Pieces<T> dz;
+        Dz dz;
 #pragma unroll
         for (int i = 0; i < 8; ++i) dz.pair(i, z[2 * i], z[2 * i + 1]);
-        second_product<T, CP>(acc, lds, dz, lane, clean);
+        second_product<NP, CP>(acc, lds, dz, lane, clean);
     };
     const int tiles = (a.n_other + 31) / 32;
     const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
@@ -230,8 +218,8 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
         auto one = [&](const char* lds, const float (*coef)[64], int tile) __attribute__((always_inline)) {
             float wv[16];
             load_weights(wv, tile);
-            const f32x16_t pr = products<T, CP>(lds, q, lane);
-            Pieces<T> dz;
+            const f32x16_t pr = products<NP, CP>(lds, q, lane);
+            Dz dz;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const Quad k4 = quad(coef, b);
@@ -242,7 +230,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
                 dz.pair(2 * b + 1, z[2], z[3]);
             }
             __builtin_amdgcn_sched_barrier(0);
-            second_product<T, CP>(acc, lds, dz, lane, CLEAN);
+            second_product<NP, CP>(acc, lds, dz, lane, CLEAN);
             add_targets(lds, coef, tile, CLEAN);
         };
         if (t0 < t1) stage(lds0, s_coef0, t0);
@@ -261,12 +249,12 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
 #pragma unroll
         for (int x = 0; x < NX; ++x) acc[x] = {};
         if (t0 >= t1) return;
-        Pieces<T> dz = {};                                             // of the tile before, whose rows are in lds3 at the start
-        for (int i = threadIdx.x * 16; i < L::BYTES; i += 4096) *(u32x4*)(lds3 + i) = u32x4{0, 0, 0, 0};
+        Dz dz = {};                                             // of the tile before, whose rows are in lds3 at the start
+        for (int i = threadIdx.x * 16; i < NP * L::BYTES; i += 4096) *(u32x4*)(lds3 + i) = u32x4{0, 0, 0, 0};
         stage(lds0, s_coef0, t0);
         if (t0 + 1 < t1) stage(lds1, s_coef1, t0 + 1);
         __syncthreads();
-        f32x16_t pr = products<T, CP>(lds0, q, lane);
+        f32x16_t pr = products<NP, CP>(lds0, q, lane);
         auto step = [&](int t, const char* before, const char* here, const char* next, char* after, const float (*coef)[64],
                         float (*coef_after)[64]) __attribute__((always_inline)) {
             __syncthreads();                                           // tile t + 1 is there; nobody reads tile t - 2 any more
@@ -274,36 +262,40 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
             float wv[16];
             load_weights(wv, t);
             f32x16_t nxt = {};
-            Pieces<T> mine;
+            Dz mine;
             float z[16];
             Quad k4 = quad(coef, 0), ahead_k4 = k4;
-            // One slice: a fragment is read (two slices ahead of its use), multiplied (in bf16, second product: by one of the two pieces), and a
-            // share of dz is computed: 16 values, then, in pairs, their pieces.  Weights may arrive during the first half of the slices.
-            constexpr int FRAGS = NKF + NX * Pieces<T>::STEPS, SLICES = NKF + NX * Pieces<T>::STEPS * Pieces<T>::N, UNITS = 24;
+            // One slice: one matrix instruction and a share of dz: 16 values, then, in pairs, their pieces.  Fragments are read two ahead.  Weights may
+            // arrive during the first half of the slices.
+            constexpr int G1 = Pairs<NP>::N, G2 = Dz::PAIRS, S1 = NKF * G1, SLICES = S1 + NX * Dz::STEPS * G2, UNITS = 24;
+            constexpr int F1 = NKF * NP, FRAGS = F1 + NX * Dz::STEPS * NP;
             u32x4 f[3];
             auto read = [&](int n) __attribute__((always_inline)) {
-                if (n < NKF) f[n % 3] = row_fragment<T, CP>(next, n, lane);
-                else if (n < FRAGS) f[n % 3] = column_fragment<T, CP>(before, (n - NKF) / NX, (n - NKF) % NX * 32, lane, false);
+                const int piece = n % NP * L::BYTES, group = (n - F1) / NP;
+                if (n < F1) f[n % 3] = row_fragment<CP>(next + piece, n / NP, lane);
+                else if (n < FRAGS) f[n % 3] = column_fragment<CP>(before + piece, group / NX, group % NX * 32, lane, false);
             };
             read(0);
             read(1);
 #pragma unroll
             for (int i = 0; i < SLICES; ++i) {
-                const int n = i < NKF ? i : NKF + (i - NKF) / Pieces<T>::N, piece = i < NKF ? 0 : (i - NKF) % Pieces<T>::N;
-                if (piece == 0) {
+                const bool one = i < S1;
+                const int group = one ? i / G1 : (i - S1) / G2, pair = one ? i % G1 : (i - S1) % G2;
+                const int n = one ? group * NP + Pairs<NP>::first(pair) : F1 + group * NP + Dz::first(pair);
+                const int second = one ? Pairs<NP>::second(pair) : Dz::second(pair);
+                if (second == 0) {
                     read(n + 2);
                     settle(f[n % 3]);
                 }
-                if (n < NKF) Wide<T>::run(nxt, f[n % 3], q[n < NKF ? n : 0]);
-                else Wide<T>::run(acc[n < NKF ? 0 : (n - NKF) % NX], f[n % 3], dz.p[n < NKF ? 0 : (n - NKF) / NX][piece]);
+                if (one) wide_mma(nxt, f[n % 3], q[one ? second : 0][one ? group : 0]);
+                else wide_mma(acc[one ? 0 : group % NX], f[n % 3], dz.p[one ? 0 : group / NX][second]);
                 const int from = GENERAL ? (2 * i < SLICES ? 0 : (2 * i - SLICES) * UNITS / SLICES) : i * UNITS / SLICES;
                 const int to = GENERAL ? (2 * i + 2 < SLICES ? 0 : (2 * i + 2 - SLICES) * UNITS / SLICES) : (i + 1) * UNITS / SLICES;
 #pragma unroll
                 for (int u = from; u < to; ++u) {
                     if (u < 16) {
-                        // f32: no registers to read ahead, and four times the matrix instructions to wait beside
-                        if (u % 4 == 0 && u > 0) k4 = OWN_BANK && F32 ? quad(coef, u / 4) : ahead_k4;
-                        if (OWN_BANK && !F32 && u % 4 == 0 && u < 12) ahead_k4 = quad(coef, u / 4 + 1);
+                        if (u % 4 == 0 && u > 0) k4 = ahead_k4;
+                        if (OWN_BANK && u % 4 == 0 && u < 12) ahead_k4 = quad(coef, u / 4 + 1);
                         z[u] = differentiate(pr, wv, k4, u, t, std::false_type{});
                         settle(z[u]);
                     } else {
@@ -328,7 +320,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
         if (t + 1 < t1) step(t + 1, lds0, lds1, lds2, lds3, s_coef1, s_coef3);
         if (t + 2 < t1) step(t + 2, lds1, lds2, lds3, lds0, s_coef2, s_coef0);
         const int last = (t1 - 1 - t0) & 3;
-        second_product<T, CP>(acc, last == 0 ? lds0 : last == 1 ? lds1 : last == 2 ? lds2 : lds3, dz, lane, false);
+        second_product<NP, CP>(acc, last == 0 ? lds0 : last == 1 ? lds1 : last == 2 ? lds2 : lds3, dz, lane, false);
     };
     if constexpr (SIDE_BY_SIDE) pass();
     else plain_pass(std::false_type{});
@@ -347,13 +339,17 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
         const int target = __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + own]);
         const float gl = a.coef[K_LOGP * n_coef + own];
         if (target >= 0 && !(GENERAL && w && w[target] == __builtin_inff())) {
-            const T* row = (const T*)a.other + (size_t)target * a.ld_other;
+            const bf16* row = a.other + (size_t)target * a.ld_other;
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int ch = x * 32 + 8 * (i >> 2) + 4 * g + (i & 3);
-                    if (ch < a.channels) acc[x][i] += gl * to_f32(row[ch]);
+                    float v = 0.0f;
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; --n)
+                        if (ch < a.channels) v += to_f32(row[n * CP + ch]);
+                    acc[x][i] += gl * v;
                 }
         }
     }
@@ -368,7 +364,7 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (ch + i < a.channels) ((T*)a.grad)[(size_t)own * a.channels + ch + i] = from_f32<T>(a.scale * acc[x][4 * b + i]);
+                    if (ch + i < a.grad_channels) ((T*)a.grad)[(size_t)own * a.grad_channels + ch + i] = from_f32<T>(a.scale * acc[x][4 * b + i]);
             }
         }
 }
@@ -376,8 +372,8 @@ __global__ __launch_bounds__(256, CP == 256 ? 1 : 2) void bank_gradient_kernel(B
 template <typename T>
 __global__ __launch_bounds__(256) void bank_gradient_join_kernel(BankArgs a, int cp) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long)a.n_own * a.channels) return;
-    const int row = (int)(id / a.channels), ch = (int)(id % a.channels);
+    if (id >= (long)a.n_own * a.grad_channels) return;
+    const int row = (int)(id / a.grad_channels), ch = (int)(id % a.grad_channels);
     float v = 0.0f;
     for (int s = 0; s < a.parts; ++s) v += a.partial[((size_t)s * a.n_own + row) * cp + ch];
     ((T*)a.grad)[id] = from_f32<T>(a.scale * v);
@@ -396,7 +392,7 @@ static void launch(const BankArgs& a, bool own_bank, hipStream_t st) {
         else hipLaunchKernelGGL((bank_gradient_kernel<T, CP, false, false>), grid, dim3(256), 0, st, a);
     }
     if (a.parts > 1)
-        hipLaunchKernelGGL((bank_gradient_join_kernel<T>), dim3((unsigned)(((long)a.n_own * a.channels + 255) / 256)), dim3(256), 0, st, a, CP);
+        hipLaunchKernelGGL((bank_gradient_join_kernel<T>), dim3((unsigned)(((long)a.n_own * a.grad_channels + 255) / 256)), dim3(256), 0, st, a, CP);
 }
 
 template <> void launch_bank_gradient<NEMO_ELEMENT>(const BankArgs& a, bool own_bank, hipStream_t st) {

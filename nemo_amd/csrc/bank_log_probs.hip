@@ -46,23 +46,55 @@ __global__ __launch_bounds__(256) void bank_coef_kernel(const float* stats, cons
     coef[K_TARGET * n + row] = __builtin_bit_cast(float, k.target);
 }
 
-// rows x cols -> rows x ld_out with the columns beyond cols zero (rows that do not start on 16 bytes).
+// Rows as the kernels take them: `rows_a` rows of one matrix, then `rows_b` of another (written behind them), channels padded with zeros to cp.
+// bf16: one piece, a copy for rows that do not start on 16 bytes.  f32: three pieces a row, each the rounding of what the ones before leave; a
+// value beyond bf16's largest is cut to it first, an infinity or NaN is the first piece alone.  Eight channels a thread.
+struct RowsOf { const void* p; long ld; int rows; };
 template <typename T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const T* src, long ld, int rows, int cols, T* dst, int ld_out) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long)rows * ld_out) return;
-    const int r = (int)(id / ld_out), c = (int)(id % ld_out);
-    dst[id] = c < cols ? src[r * ld + c] : (T)0.0f;
+__global__ __launch_bounds__(256) void bank_rows_kernel(RowsOf a, RowsOf b, int channels, int cp, bf16* out_a, bf16* out_b) {
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+    const uint32_t per_row = cp / 8, id = blockIdx.x * 256u + threadIdx.x;          // fewer than 2^31 threads: see check_bank
+    const uint32_t r = id / per_row;
+    const int c = (int)(id - r * per_row) * 8;
+    if (r >= (uint32_t)(a.rows + b.rows)) return;
+    const bool second = r >= (uint32_t)a.rows;
+    const long row = second ? r - a.rows : r;
+    const T* src = (const T*)(second ? b.p : a.p) + row * (second ? b.ld : a.ld) + c;
+    bf16* dst = (second ? out_b : out_a) + row * (long)(NP * cp) + c;
+    float v[8] = {};
+    if (c + 8 <= channels) {
+        const typename Loose<T, 8>::V t = load_loose<8>(src);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < channels) v[i] = to_f32(src[i]);
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        bf16x8 piece;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float most = 3.3895313892515355e38f;
+            float h = (float)(bf16)v[i];
+            if (NP > 1 && n == 0 && __builtin_fabsf(v[i]) > most && __builtin_fabsf(v[i]) <= FLT_MAX) h = v[i] > 0.0f ? most : -most;
+            piece[i] = (bf16)h;
+            v[i] = __builtin_fabsf(h) <= FLT_MAX ? v[i] - h : 0.0f;
+        }
+        *(bf16x8*)(dst + n * cp) = piece;
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-static int elem(int dtype) { return dtype == NEMO_F32 ? 4 : 2; }
 static bool aligned_rows(const void* p, int64_t ld, int64_t cols, int es) {
     return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && (cols * es) % 16 == 0;
 }
-static size_t pack_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
-    return aligned_rows(p, ld, cols, elem(dtype)) ? 0 : align256((size_t)rows * padded_channels((int)cols) * elem(dtype));
+// Bytes of the rows' copy in the workspace.
+static size_t rows_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+    if (dtype == NEMO_BF16 && aligned_rows(p, ld, cols, 2)) return 0;
+    return align256((size_t)rows * padded_channels((int)cols) * 2 * (dtype == NEMO_F32 ? 3 : 1));
 }
 
 // Parts of the other axis: `per_cu` workgroups a compute unit (what a kernel's registers leave room for), at least four tiles a part, at most 32.
@@ -76,8 +108,12 @@ static Parts parts_of_bank(int64_t owners, int64_t others, int per_cu) {
     const int64_t per = tiles > 0 ? (tiles + p - 1) / p : 1;
     return {(int)(tiles > 0 ? (tiles + per - 1) / per : 1), (int)per};
 }
-static Parts forward_parts(int64_t rows, int64_t cols, int cp, int es) { return parts_of_bank(rows, cols, cp * es <= 256 ? 4 : 2); }
-static Parts gradient_parts(int64_t owners, int64_t others, int cp) { return parts_of_bank(owners, others, cp == 256 ? 1 : 2); }
+static Parts forward_parts(int64_t rows, int64_t cols, int cp, int dtype) {
+    return parts_of_bank(rows, cols, dtype == NEMO_F32 ? (cp == 64 ? 3 : cp == 128 ? 2 : 1) : cp <= 128 ? 4 : 2);
+}
+static Parts gradient_parts(int64_t owners, int64_t others, int cp, int dtype) {
+    return parts_of_bank(owners, others, dtype == NEMO_F32 ? (cp == 64 ? 2 : 1) : cp <= 128 ? 2 : 1);
+}
 
 // The state's form: 0 where it is kept of the scores, else what turns a product into its score in units of log 2.
 static float product_unit(const float* weights, float scale, int top) {
@@ -94,18 +130,25 @@ static int check_bank(const char* who, int64_t rows, int64_t cols, int64_t chann
     return NEMO_OK;
 }
 
-struct RowsIn { const void* p; int64_t ld; };
-static RowsIn rows_in(int dtype, const void* p, int64_t ld, int64_t rows, int64_t cols, char*& ws, hipStream_t st) {
-    if (aligned_rows(p, ld, cols, elem(dtype)) || rows == 0) return {p, ld};
-    const int cp = padded_channels((int)cols);
-    void* dst = ws;
-    ws += pack_bytes(p, ld, rows, cols, dtype);
-    const unsigned wgs = (unsigned)((rows * cp + 255) / 256);
+struct RowsIn { const bf16* p; int64_t ld; };
+static void rows_in(int dtype, const void* features, int64_t ldf, int64_t rows, const void* bank, int64_t ldb, int64_t cols, int64_t channels,
+                    char*& ws, hipStream_t st, RowsIn* f, RowsIn* b) {
+    const int cp = padded_channels((int)channels);
+    *f = {(const bf16*)features, ldf};
+    *b = {(const bf16*)bank, ldb};
+    const size_t bytes_f = rows_bytes(features, ldf, rows, channels, dtype), bytes_b = rows_bytes(bank, ldb, cols, channels, dtype);
+    const int64_t ld_out = (int64_t)cp * (dtype == NEMO_F32 ? 3 : 1);
+    if (bytes_f) *f = {(bf16*)ws, ld_out};
+    if (bytes_b) *b = {(bf16*)(ws + bytes_f), ld_out};
+    ws += bytes_f + bytes_b;
+    const int na = bytes_f ? (int)rows : 0, nb = bytes_b ? (int)cols : 0;
+    if (na + nb == 0) return;
+    const unsigned wgs = (unsigned)(((int64_t)(na + nb) * (cp / 8) + 255) / 256);
+    const RowsOf ra = {features, (long)ldf, na}, rb = {bank, (long)ldb, nb};
     if (dtype == NEMO_F32)
-        hipLaunchKernelGGL((pack_rows_kernel<float>), dim3(wgs), dim3(256), 0, st, (const float*)p, ld, (int)rows, (int)cols, (float*)dst, cp);
+        hipLaunchKernelGGL((bank_rows_kernel<float>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p);
     else
-        hipLaunchKernelGGL((pack_rows_kernel<bf16>), dim3(wgs), dim3(256), 0, st, (const bf16*)p, ld, (int)rows, (int)cols, (bf16*)dst, cp);
-    return {dst, cp};
+        hipLaunchKernelGGL((bank_rows_kernel<bf16>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p);
 }
 
 }  // namespace nemo
@@ -115,8 +158,8 @@ using namespace nemo;
 extern "C" size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                                 int64_t channels, int32_t dtype, int32_t top) {
     if (rows <= 0 || cols < 0 || channels <= 0 || channels > 256) return 0;
-    const Parts p = forward_parts(rows, cols, padded_channels((int)channels), elem(dtype));
-    return pack_bytes(features, ldf, rows, channels, dtype) + pack_bytes(bank, ldb, cols, channels, dtype) +
+    const Parts p = forward_parts(rows, cols, padded_channels((int)channels), dtype);
+    return rows_bytes(features, ldf, rows, channels, dtype) + rows_bytes(bank, ldb, cols, channels, dtype) +
            align256((size_t)3 * 2 * p.parts * rows * 4) + 2 * align256((size_t)2 * p.parts * rows * top * 4) + align256((size_t)rows * 4);
 }
 
@@ -137,12 +180,13 @@ extern "C" int nemo_bank_log_probs(const void* features, int64_t ldf, const void
         return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    const RowsIn f = rows_in(dtype, features, ldf, rows, channels, ws, st), b = rows_in(dtype, bank, ldb, cols, channels, ws, st);
-    const Parts p = forward_parts(rows, cols, padded_channels((int)channels), elem(dtype));
+    RowsIn f, b;
+    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st, &f, &b);
+    const Parts p = forward_parts(rows, cols, padded_channels((int)channels), dtype);
     BankArgs a = {};
     a.own = f.p; a.ld_own = f.ld; a.n_own = (int)rows;
     a.other = b.p; a.ld_other = b.ld; a.n_other = (int)cols;
-    a.channels = (int)channels;
+    a.channels = (int)(channels + 7) / 8 * 8;
     a.weights = weights; a.ldw = ldw; a.targets = (const long long*)targets; a.scale = scale;
     a.parts = p.parts; a.part_tiles = p.tiles;
     a.part_state = (float*)ws;
@@ -164,9 +208,9 @@ extern "C" size_t nemo_bank_log_probs_backward_workspace(const void* features, i
                                                          int64_t cols, int64_t channels, int32_t dtype) {
     if (rows <= 0 || cols <= 0 || channels <= 0 || channels > 256) return 0;
     const int cp = padded_channels((int)channels);
-    const Parts pf = gradient_parts(rows, cols, cp), pb = gradient_parts(cols, rows, cp);
+    const Parts pf = gradient_parts(rows, cols, cp, dtype), pb = gradient_parts(cols, rows, cp, dtype);
     const size_t bf = pf.parts > 1 ? (size_t)pf.parts * rows * cp * 4 : 0, bb = pb.parts > 1 ? (size_t)pb.parts * cols * cp * 4 : 0;
-    return pack_bytes(features, ldf, rows, channels, dtype) + pack_bytes(bank, ldb, cols, channels, dtype) + align256((size_t)K_COUNT * coef_rows(rows) * 4) +
+    return rows_bytes(features, ldf, rows, channels, dtype) + rows_bytes(bank, ldb, cols, channels, dtype) + align256((size_t)K_COUNT * coef_rows(rows) * 4) +
            align256(bf > bb ? bf : bb);
 }
 
@@ -187,7 +231,8 @@ extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, c
         return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    const RowsIn f = rows_in(dtype, features, ldf, rows, channels, ws, st), b = rows_in(dtype, bank, ldb, cols, channels, ws, st);
+    RowsIn f, b;
+    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st, &f, &b);
     float* coef = (float*)ws;
     ws += align256((size_t)K_COUNT * coef_rows(rows) * 4);
     const float unit = product_unit(weights, scale, top);
@@ -199,11 +244,12 @@ extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, c
         if (!grad) continue;
         const RowsIn own = own_bank ? b : f, other = own_bank ? f : b;
         const int64_t n_own = own_bank ? cols : rows, n_other = own_bank ? rows : cols;
-        const Parts p = gradient_parts(n_own, n_other, cp);
+        const Parts p = gradient_parts(n_own, n_other, cp, dtype);
         BankArgs a = {};
         a.own = own.p; a.ld_own = own.ld; a.n_own = (int)n_own;
         a.other = other.p; a.ld_other = other.ld; a.n_other = (int)n_other;
-        a.channels = (int)channels;
+        a.channels = (int)(channels + 7) / 8 * 8;
+        a.grad_channels = (int)channels;
         a.weights = weights; a.ldw = ldw; a.targets = (const long long*)targets; a.scale = scale;
         a.parts = p.parts; a.part_tiles = p.tiles;
         a.out.k = unit;
