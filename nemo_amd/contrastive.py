@@ -13,10 +13,10 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
-def _device_tensors(what, dtypes, **tensors):
+def _device_tensors(what, dtypes, names, *tensors):
     """All tensors on one GPU and of one of `dtypes` (None entries are skipped)."""
-    first = None
-    for name, t in tensors.items():
+    first = tensors[0]
+    for name, t in zip(names, tensors):
         if t is None:
             continue
         if not torch.is_tensor(t):
@@ -25,12 +25,14 @@ def _device_tensors(what, dtypes, **tensors):
             raise RuntimeError(f"{what}: {name} is a CPU tensor; nemo_amd kernels need device tensors, there is no CPU path")
         if t.dtype not in dtypes:
             raise TypeError(f"{what}: {name} is {t.dtype}, takes {', '.join(str(d) for d in dtypes)}")
-        if first is None:
-            first = (name, t)
-        elif t.device != first[1].device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, {first[0]} on {first[1].device}")
-        elif t.dtype != first[1].dtype:
-            raise TypeError(f"{what}: {name} is {t.dtype}, {first[0]} {first[1].dtype}")
+        if t is not first and t.device != first.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, {names[0]} on {first.device}")
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what}: {name} is {t.dtype}, {names[0]} {first.dtype}")
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _number(what, name, value):
@@ -76,7 +78,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     activation: "none", "relu", "gelu" (the exact one, with erf) or "silu".  Products are summed in 32 bits (float32: on the f32 matrix
     cores, so infinities and NaN come out as in any f32 product) and the result is rounded once.  x, weight, bias and residual are
     differentiable.  Rows of x, weight and residual may be strided; alignment matters for speed only."""
-    _device_tensors("linear", tuple(ops.DTYPES), x=x, weight=weight, bias=bias, residual=residual)
+    _device_tensors("linear", ops.DTYPES, ("x", "weight", "bias", "residual"), x, weight, bias, residual)
     if activation not in ops.ACTIVATIONS:
         raise ValueError(f"linear: activation {activation!r} (takes {', '.join(ops.ACTIVATIONS)})")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
@@ -91,8 +93,13 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     M = 1
     for n in lead:
         M *= n
-    y = _Linear.apply(x.reshape(M, K), weight, bias, None if residual is None else residual.reshape(M, N), activation, alpha, beta)
-    return y.reshape(lead + (N,))
+    if x.dim() != 2:
+        x, residual = x.reshape(M, K), None if residual is None else residual.reshape(M, N)
+    if _wants_grad(x, weight, bias, residual):
+        y = _Linear.apply(x, weight, bias, residual, activation, alpha, beta)
+    else:
+        y, _ = ops.linear(x, weight, bias, residual, activation, alpha, beta)
+    return y if len(lead) == 1 else y.reshape(lead + (N,))
 
 
 LogProbs = namedtuple("LogProbs", "logp entropy lse top_logp top_index")
@@ -110,7 +117,7 @@ def _probs_arguments(what, rows, cols, device, targets, weights, scale, top):
         if targets.numel() and (int(targets.min()) < -1 or int(targets.max()) >= cols):      # on the host: nothing to wait for
             raise ValueError(f"{what}: targets must lie in -1 .. {cols - 1}")
     if weights is not None:
-        _device_tensors(what, (torch.float32,), weights=weights)
+        _device_tensors(what, (torch.float32,), ("weights",), weights)
         if weights.device != device:
             raise RuntimeError(f"{what}: weights are on {weights.device}, the rows on {device}")
         if tuple(weights.shape) not in ((cols,), (rows, cols)):
@@ -119,19 +126,25 @@ def _probs_arguments(what, rows, cols, device, targets, weights, scale, top):
             raise ValueError(f"{what}: weights are constants, they get no gradient: pass weights.detach()")
     if isinstance(top, bool) or int(top) != top or not 0 <= top <= 16:
         raise ValueError(f"{what}: top must be a whole number in 0 .. 16, got {top}")
-    return targets.to(device=device, dtype=torch.int64), _number(what, "scale", scale), int(top)
+    if targets.dtype != torch.int64 or targets.device != device:
+        targets = targets.to(device=device, dtype=torch.int64)
+    return targets, _number(what, "scale", scale), int(top)
+
+
+def _results(out):
+    return out.logp, out.entropy, out.lse, out.top_logp, out.top_index
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, weights, scale, top):
-        out, stats, top_logp, top_index = ops.log_probs(logits, targets, weights, scale, top)
-        ctx.save_for_backward(logits, targets, weights, stats)
+        out = ops.log_probs(logits, targets, weights, scale, top)
+        ctx.save_for_backward(logits, targets, weights, out.stats)
         ctx.scale = scale
         if top:
-            ctx.mark_non_differentiable(top_logp, top_index)
+            ctx.mark_non_differentiable(out.top_logp, out.top_index)
         ctx.set_materialize_grads(False)
-        return out[0], out[1], out[2], top_logp, top_index
+        return _results(out)
 
     @staticmethod
     @once_differentiable
@@ -154,24 +167,26 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0):
     back.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place out, whatever the logit there is (NaN
     too).  A row with nothing left: lse and logp -inf, entropy 0, top_index -1, gradient 0.  A row with a NaN or +inf left: NaN,
     top_index -1.  Fewer places left than `top`: -inf and -1 in their stead."""
-    _device_tensors("log_probs", tuple(ops.DTYPES), logits=logits)
+    _device_tensors("log_probs", ops.DTYPES, ("logits",), logits)
     if logits.dim() != 2:
         raise ValueError(f"log_probs: logits must be [S, V], got {tuple(logits.shape)}")
     S, V = logits.shape
     targets, scale, top = _probs_arguments("log_probs", S, V, logits.device, targets, weights, scale, top)
-    return LogProbs(*_LogProbs.apply(logits, targets, weights, scale, top))
+    if _wants_grad(logits):
+        return LogProbs(*_LogProbs.apply(logits, targets, weights, scale, top))
+    return LogProbs(*_results(ops.log_probs(logits, targets, weights, scale, top, want_stats=False)))
 
 
 class _BankLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, bank, targets, weights, scale, top):
-        out, stats, top_logp, top_index = ops.bank_log_probs(features, bank, targets, weights, scale, top)
-        ctx.save_for_backward(features, bank, targets, weights, stats)
+        out = ops.bank_log_probs(features, bank, targets, weights, scale, top)
+        ctx.save_for_backward(features, bank, targets, weights, out.stats)
         ctx.scale, ctx.top = scale, top
         if top:
-            ctx.mark_non_differentiable(top_logp, top_index)
+            ctx.mark_non_differentiable(out.top_logp, out.top_index)
         ctx.set_materialize_grads(False)
-        return out[0], out[1], out[2], top_logp, top_index
+        return _results(out)
 
     @staticmethod
     @once_differentiable
@@ -188,11 +203,13 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
     """log_probs(linear(features, bank), ...) without the [S, V] matrix: features [S, C] and bank [V, C], both float32 or both bfloat16, C up
     to 256.  Scores are z = scale <feature, bank row> - weights, summed in 32 bits; arguments, results and rules are those of log_probs.
     Differentiable with respect to features and bank; the gradient computes the scores again instead of keeping them."""
-    _device_tensors("bank_log_probs", (torch.float32, torch.bfloat16), features=features, bank=bank)
+    _device_tensors("bank_log_probs", (torch.float32, torch.bfloat16), ("features", "bank"), features, bank)
     if features.dim() != 2 or bank.dim() != 2 or features.shape[1] != bank.shape[1]:
         raise ValueError(f"bank_log_probs: features must be [S, C] and bank [V, C], got {tuple(features.shape)} and {tuple(bank.shape)}")
     if not 1 <= features.shape[1] <= 256:
         raise ValueError(f"bank_log_probs: {features.shape[1]} channels (takes 1 to 256: use linear and log_probs)")
     S, V = features.shape[0], bank.shape[0]
     targets, scale, top = _probs_arguments("bank_log_probs", S, V, features.device, targets, weights, scale, top)
-    return LogProbs(*_BankLogProbs.apply(features, bank, targets, weights, scale, top))
+    if _wants_grad(features, bank):
+        return LogProbs(*_BankLogProbs.apply(features, bank, targets, weights, scale, top))
+    return LogProbs(*_results(ops.bank_log_probs(features, bank, targets, weights, scale, top, want_stats=False)))

@@ -339,17 +339,24 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
         const int target = __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + own]);
         const float gl = a.coef[K_LOGP * n_coef + own];
         if (target >= 0 && !(GENERAL && w && w[target] == __builtin_inff())) {
-            const bf16* row = a.other + (size_t)target * a.ld_other;
+            const bf16* row = a.other + (size_t)target * a.ld_other + 4 * g;
+            typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int ch = x * 32 + 8 * (i >> 2) + 4 * g + (i & 3);
-                    float v = 0.0f;
+                for (int b = 0; b < 4; ++b) {
+                    const int ch = x * 32 + 8 * b;
+                    if (ch >= a.channels) continue;
+                    bf16x4 v[NP];                                      // rows start on 16 bytes
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; --n)
-                        if (ch < a.channels) v += to_f32(row[n * CP + ch]);
-                    acc[x][i] += gl * v;
+                    for (int n = 0; n < NP; ++n) v[n] = *(const bf16x4*)(row + n * CP + ch);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) sum += to_f32(v[n][i]);
+                        acc[x][4 * b + i] += gl * sum;
+                    }
                 }
         }
     }
@@ -362,18 +369,24 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
                 *(f32x4*)(a.partial + ((size_t)part * a.n_own + own) * CP + ch) =
                     (f32x4){acc[x][4 * b], acc[x][4 * b + 1], acc[x][4 * b + 2], acc[x][4 * b + 3]};
             } else {
+                T* at = (T*)a.grad + (size_t)own * a.grad_channels + ch;
+                typename Loose<T, 4>::V v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (ch + i < a.grad_channels) ((T*)a.grad)[(size_t)own * a.grad_channels + ch + i] = from_f32<T>(a.scale * acc[x][4 * b + i]);
+                for (int i = 0; i < 4; ++i) v[i] = from_f32<T>(a.scale * acc[x][4 * b + i]);
+                if (ch + 4 <= a.grad_channels) store_loose<4>(at, v);
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (ch + i < a.grad_channels) at[i] = v[i];
             }
         }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void bank_gradient_join_kernel(BankArgs a, int cp) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long)a.n_own * a.grad_channels) return;
-    const int row = (int)(id / a.grad_channels), ch = (int)(id % a.grad_channels);
+    const uint32_t id = blockIdx.x * 256u + threadIdx.x;               // fewer than 2^24 rows of at most 256 channels
+    if (id >= (uint32_t)a.n_own * (uint32_t)a.grad_channels) return;
+    const uint32_t row = id / (uint32_t)a.grad_channels, ch = id - row * (uint32_t)a.grad_channels;
     float v = 0.0f;
     for (int s = 0; s < a.parts; ++s) v += a.partial[((size_t)s * a.n_own + row) * cp + ch];
     ((T*)a.grad)[id] = from_f32<T>(a.scale * v);

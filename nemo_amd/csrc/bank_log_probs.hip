@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/nemo_hip.h"
 #include "bank_tiles.h"
 #include "errors.h"
@@ -32,28 +34,37 @@ __global__ __launch_bounds__(256) void bank_join_kernel(BankArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void bank_coef_kernel(const float* stats, const float* g_logp, const float* g_entropy, const float* g_lse,
-                                                        const long long* targets, int rows, int cols, float* coef, bool join_m) {
-    const int row = blockIdx.x * 256 + threadIdx.x, n = coef_rows(rows);
+// What the gradients need of a row, as arrays over the rows; the rows behind the last, up to whole tiles, give nothing.
+struct CoefArgs {
+    const float *stats, *g_logp, *g_entropy, *g_lse;
+    const long long* targets;
+    float* coef;
+    int rows, cols;
+    bool join_m;
+};
+__device__ void write_coef(const CoefArgs& a, int row) {
+    const int n = coef_rows(a.rows);
     if (row >= n) return;
     RowCoef k = {0.0f, kNoProbability, 0.0f, 0.0f, 0.0f, -1};
-    if (row < rows) k = row_coef(stats, g_logp, g_entropy, g_lse, targets, row, cols);
-    coef[K_M * n + row] = join_m ? k.m + k.log2_s : k.m;
-    coef[K_LOG2_S * n + row] = k.log2_s;
-    coef[K_C * n + row] = k.c;
-    coef[K_G2 * n + row] = k.g2;
-    coef[K_LOGP * n + row] = k.g_logp;
-    coef[K_TARGET * n + row] = __builtin_bit_cast(float, k.target);
+    if (row < a.rows) k = row_coef(a.stats, a.g_logp, a.g_entropy, a.g_lse, a.targets, row, a.cols);
+    a.coef[K_M * n + row] = a.join_m ? k.m + k.log2_s : k.m;
+    a.coef[K_LOG2_S * n + row] = k.log2_s;
+    a.coef[K_C * n + row] = k.c;
+    a.coef[K_G2 * n + row] = k.g2;
+    a.coef[K_LOGP * n + row] = k.g_logp;
+    a.coef[K_TARGET * n + row] = __builtin_bit_cast(float, k.target);
 }
 
 // Rows as the kernels take them: `rows_a` rows of one matrix, then `rows_b` of another (written behind them), channels padded with zeros to cp.
 // bf16: one piece, a copy for rows that do not start on 16 bytes.  f32: three pieces a row, each the rounding of what the ones before leave; a
 // value beyond bf16's largest is cut to it first, an infinity or NaN is the first piece alone.  Eight channels a thread.
+// The first workgroups write the coefficients instead (a backward call's; none in a forward call): one launch for all that comes before.
 struct RowsOf { const void* p; long ld; int rows; };
 template <typename T>
-__global__ __launch_bounds__(256) void bank_rows_kernel(RowsOf a, RowsOf b, int channels, int cp, bf16* out_a, bf16* out_b) {
+__global__ __launch_bounds__(256) void bank_rows_kernel(RowsOf a, RowsOf b, int channels, int cp, bf16* out_a, bf16* out_b, CoefArgs k, uint32_t k_groups) {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-    const uint32_t per_row = cp / 8, id = blockIdx.x * 256u + threadIdx.x;          // fewer than 2^31 threads: see check_bank
+    if (blockIdx.x < k_groups) return write_coef(k, (int)(blockIdx.x * 256 + threadIdx.x));
+    const uint32_t per_row = cp / 8, id = (blockIdx.x - k_groups) * 256u + threadIdx.x;          // fewer than 2^31 threads: see check_bank
     const uint32_t r = id / per_row;
     const int c = (int)(id - r * per_row) * 8;
     if (r >= (uint32_t)(a.rows + b.rows)) return;
@@ -97,22 +108,23 @@ static size_t rows_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, 
     return align256((size_t)rows * padded_channels((int)cols) * 2 * (dtype == NEMO_F32 ? 3 : 1));
 }
 
-// Parts of the other axis: `per_cu` workgroups a compute unit (what a kernel's registers leave room for), at least four tiles a part, at most 32.
+// Parts of the other axis, at most 32: while the card is not full, parts down to `least` tiles, a workgroup a compute unit; beyond that
+// `per_cu` workgroups a unit (what a kernel's registers leave room for), of at least four tiles.  Measured (a call in us, f32, 128 channels,
+// parts of one tile / four): forward 17 rows of 643 11.3 / 17.1, 1000 of 1000 16.2 / 20.3, 4096 of 643 26.5 / 25.1; backward, whose parts
+// are written out and joined, with two tiles / four / one: 128 of 1024 72 / 86 / 71, 1000 of 1000 81 / 88 / 90.
 struct Parts { int parts, tiles; };
-static Parts parts_of_bank(int64_t owners, int64_t others, int per_cu) {
-    const int64_t groups = (owners + 127) / 128, tiles = (others + 31) / 32;
-    int64_t p = groups > 0 ? 256 * per_cu / groups : 1;
-    if (p > tiles / 4) p = tiles / 4;
-    if (p > 32) p = 32;
-    if (p < 1) p = 1;
+static Parts parts_of_bank(int64_t owners, int64_t others, int per_cu, int least) {
+    const int64_t groups = owners > 0 ? (owners + 127) / 128 : 1, tiles = (others + 31) / 32;
+    const int64_t few = std::min(256 / groups, tiles / least), many = std::min(256 * per_cu / groups, tiles / 4);
+    const int64_t p = std::max<int64_t>(1, std::min<int64_t>(32, std::max(few, many)));
     const int64_t per = tiles > 0 ? (tiles + p - 1) / p : 1;
     return {(int)(tiles > 0 ? (tiles + per - 1) / per : 1), (int)per};
 }
 static Parts forward_parts(int64_t rows, int64_t cols, int cp, int dtype) {
-    return parts_of_bank(rows, cols, dtype == NEMO_F32 ? (cp == 64 ? 3 : cp == 128 ? 2 : 1) : cp <= 128 ? 4 : 2);
+    return parts_of_bank(rows, cols, dtype == NEMO_F32 ? (cp == 64 ? 3 : cp == 128 ? 2 : 1) : cp <= 128 ? 4 : 2, 1);
 }
 static Parts gradient_parts(int64_t owners, int64_t others, int cp, int dtype) {
-    return parts_of_bank(owners, others, dtype == NEMO_F32 ? (cp == 64 ? 2 : 1) : cp <= 128 ? 2 : 1);
+    return parts_of_bank(owners, others, dtype == NEMO_F32 ? (cp == 64 ? 2 : 1) : cp <= 128 ? 2 : 1, 2);
 }
 
 // The state's form: 0 where it is kept of the scores, else what turns a product into its score in units of log 2.
@@ -132,7 +144,7 @@ static int check_bank(const char* who, int64_t rows, int64_t cols, int64_t chann
 
 struct RowsIn { const bf16* p; int64_t ld; };
 static void rows_in(int dtype, const void* features, int64_t ldf, int64_t rows, const void* bank, int64_t ldb, int64_t cols, int64_t channels,
-                    char*& ws, hipStream_t st, RowsIn* f, RowsIn* b) {
+                    char*& ws, hipStream_t st, const CoefArgs& k, RowsIn* f, RowsIn* b) {
     const int cp = padded_channels((int)channels);
     *f = {(const bf16*)features, ldf};
     *b = {(const bf16*)bank, ldb};
@@ -142,13 +154,14 @@ static void rows_in(int dtype, const void* features, int64_t ldf, int64_t rows, 
     if (bytes_b) *b = {(bf16*)(ws + bytes_f), ld_out};
     ws += bytes_f + bytes_b;
     const int na = bytes_f ? (int)rows : 0, nb = bytes_b ? (int)cols : 0;
-    if (na + nb == 0) return;
-    const unsigned wgs = (unsigned)(((int64_t)(na + nb) * (cp / 8) + 255) / 256);
+    const unsigned k_groups = k.coef ? (unsigned)(coef_rows(k.rows) + 255) / 256 : 0;
+    const unsigned wgs = k_groups + (unsigned)(((int64_t)(na + nb) * (cp / 8) + 255) / 256);
+    if (wgs == 0) return;
     const RowsOf ra = {features, (long)ldf, na}, rb = {bank, (long)ldb, nb};
     if (dtype == NEMO_F32)
-        hipLaunchKernelGGL((bank_rows_kernel<float>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p);
+        hipLaunchKernelGGL((bank_rows_kernel<float>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p, k, k_groups);
     else
-        hipLaunchKernelGGL((bank_rows_kernel<bf16>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p);
+        hipLaunchKernelGGL((bank_rows_kernel<bf16>), dim3(wgs), dim3(256), 0, st, ra, rb, (int)channels, cp, (bf16*)f->p, (bf16*)b->p, k, k_groups);
 }
 
 }  // namespace nemo
@@ -181,7 +194,7 @@ extern "C" int nemo_bank_log_probs(const void* features, int64_t ldf, const void
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     RowsIn f, b;
-    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st, &f, &b);
+    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st, CoefArgs{}, &f, &b);
     const Parts p = forward_parts(rows, cols, padded_channels((int)channels), dtype);
     BankArgs a = {};
     a.own = f.p; a.ld_own = f.ld; a.n_own = (int)rows;
@@ -231,13 +244,12 @@ extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, c
         return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    RowsIn f, b;
-    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st, &f, &b);
+    const float unit = product_unit(weights, scale, top);
     float* coef = (float*)ws;
     ws += align256((size_t)K_COUNT * coef_rows(rows) * 4);
-    const float unit = product_unit(weights, scale, top);
-    hipLaunchKernelGGL(bank_coef_kernel, dim3((unsigned)((coef_rows(rows) + 255) / 256)), dim3(256), 0, st, stats, g_logp, g_entropy, g_lse,
-                       (const long long*)targets, (int)rows, (int)cols, coef, unit != 0.0f && dtype == NEMO_BF16);
+    RowsIn f, b;
+    rows_in(dtype, features, ldf, rows, bank, ldb, cols, channels, ws, st,
+            {stats, g_logp, g_entropy, g_lse, (const long long*)targets, coef, (int)rows, (int)cols, unit != 0.0f && dtype == NEMO_BF16}, &f, &b);
     const int cp = padded_channels((int)channels);
     for (int own_bank = 0; own_bank < 2; ++own_bank) {
         void* grad = own_bank ? grad_bank : grad_features;

@@ -3,6 +3,7 @@
 Each wrapper allocates its outputs with torch (device memory plumbing), passes raw pointers and the
 current stream, and raises on a non-zero return code.  No arithmetic happens here.
 """
+import contextlib
 import ctypes as C
 
 import torch
@@ -690,31 +691,41 @@ def spherical_angles(campos):
 
 
 # ---- the contrastive loss of the feature bank (contrastive.py adds autograd and the checks of its arguments) ----
+# Small calls are bound by the host: pointers go to ctypes as integers, the device is switched only where it differs, the stream is asked
+# for without a wrapper object.
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_SAME_DEVICE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _on(device):
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def rows_2d(t, width):
     """(t as [rows, width] whose rows are contiguous, row stride in elements): a view where the strides allow it, else a copy.
     Rows may lie apart (a slice of wider rows); overlapping or permuted ones are copied."""
-    t = t.detach()
     if t.dim() != 2:
         rows = 1
         for n in t.shape[:-1]:
             rows *= n
-        t = t.reshape(rows, width)
-    if t.is_contiguous() or t.numel() == 0:
+        t = t.detach().reshape(rows, width)
+    if t.is_contiguous():
+        return t, width
+    if t.numel() == 0:
         return t, width
     if (width == 1 or t.stride(1) == 1) and t.stride(0) >= width:
         return t, t.stride(0)
-    return t.contiguous(), width
+    return t.detach().contiguous(), width
 
 
 def _raw(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _scratch(nbytes, device):
+    """Workspace of a call; freed after it, which on one stream is in order."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
@@ -727,16 +738,17 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     ldr = N
     if residual is not None:
         residual, ldr = rows_2d(residual, N)
-    if bias is not None:
+    if bias is not None and not bias.is_contiguous():
         bias = bias.detach().contiguous()
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    pre = torch.empty(M, N, dtype=x.dtype, device=x.device) if want_pre else None
-    dt = DTYPES[x.dtype]
-    with torch.cuda.device(x.device):
-        nbytes = lib.nemo_linear_workspace(_raw(x), ldx, _raw(weight), ldw, M, N, K, dt)
-        ws = _scratch(nbytes, x.device)
-        check(lib.nemo_linear(_raw(x), ldx, _raw(weight), ldw, _raw(bias), _raw(residual), ldr, M, N, K, dt, ACTIVATIONS[activation],
-                              float(alpha), float(beta), _raw(y), _raw(pre), _raw(ws), nbytes, stream_ptr()), "nemo_linear")
+    dev, dt = x.device, DTYPES[x.dtype]
+    y = torch.empty((M, N), dtype=x.dtype, device=dev)
+    pre = torch.empty((M, N), dtype=x.dtype, device=dev) if want_pre else None
+    px, pw = x.data_ptr(), weight.data_ptr()
+    with _on(dev):
+        nbytes = lib.nemo_linear_workspace(px, ldx, pw, ldw, M, N, K, dt)
+        ws = _scratch(nbytes, dev)
+        check(lib.nemo_linear(px, ldx, pw, ldw, _raw(bias), _raw(residual), ldr, M, N, K, dt, ACTIVATIONS[activation], alpha, beta, y.data_ptr(),
+                              _raw(pre), _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_linear")
     return y, pre
 
 
@@ -752,12 +764,12 @@ def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1
     shapes = ((M, K), (N, K), (N,), (M, N))
     empty = torch.zeros if M == 0 or N == 0 else torch.empty                # a sum over nothing is zero
     outs = [empty(s, dtype=grad_y.dtype, device=dev) if w else None for s, w in zip(shapes, want)]
-    with torch.cuda.device(dev):
-        nbytes = lib.nemo_linear_backward_workspace(_raw(grad_y), ldg, _raw(x), ldx, _raw(weight), ldw, M, N, K, dt, ACTIVATIONS[activation])
+    pg, px, pw, act = grad_y.data_ptr(), _raw(x), _raw(weight), ACTIVATIONS[activation]
+    with _on(dev):
+        nbytes = lib.nemo_linear_backward_workspace(pg, ldg, px, ldx, pw, ldw, M, N, K, dt, act)
         ws = _scratch(nbytes, dev)
-        check(lib.nemo_linear_backward(_raw(grad_y), ldg, _raw(x), ldx, _raw(weight), ldw, _raw(pre), M, N, K, dt, ACTIVATIONS[activation],
-                                       float(alpha), float(beta), *[_raw(o) for o in outs], _raw(ws), nbytes, stream_ptr()),
-              "nemo_linear_backward")
+        check(lib.nemo_linear_backward(pg, ldg, px, ldx, pw, ldw, _raw(pre), M, N, K, dt, act, alpha, beta, *[_raw(o) for o in outs], _raw(ws),
+                                       nbytes, _raw_stream(dev.index)), "nemo_linear_backward")
     return tuple(outs)
 
 
@@ -766,53 +778,64 @@ def _row_weights(weights, cols):
     if weights is None:
         return None, 0
     if weights.dim() == 1:
-        return weights.detach().contiguous(), 0
+        return weights.contiguous(), 0
     return rows_2d(weights, cols)
 
 
-def _log_probs_outputs(rows, top, device):
-    out = torch.empty(3, rows, device=device)
-    stats = torch.empty(rows, 4, device=device)
-    top_logp = torch.empty(rows, top, device=device) if top else None
-    top_index = torch.empty(rows, top, dtype=torch.int64, device=device) if top else None
-    return out, stats, top_logp, top_index
+def _f32_row(g):
+    """A gradient [S] as contiguous f32, or None."""
+    return None if g is None else g.detach().to(torch.float32).contiguous() if g.dtype != torch.float32 or not g.is_contiguous() else g
 
 
-def log_probs(logits, targets, weights=None, scale=1.0, top=0):
-    """logits [S,V], targets [S] i64, weights None / [V] / [S,V] f32 -> (out [3,S] = logp, entropy, lse; stats [S,4] for the backward
-    call; top_logp [S,top], top_index [S,top] i64, or None, None)."""
+class _Probs:
+    """Outputs of a log-prob call: logp, entropy, lse [S] f32; stats [S,4] for the backward call (None unless wanted); top_logp [S,top],
+    top_index [S,top] i64 (None for top = 0)."""
+
+    def __init__(self, rows, top, want_stats, device):
+        self.logp, self.entropy, self.lse = [torch.empty(rows, device=device) for _ in range(3)]
+        self.stats = torch.empty((rows, 4), device=device) if want_stats else None
+        self.top_logp = torch.empty((rows, top), device=device) if top else None
+        self.top_index = torch.empty((rows, top), dtype=torch.int64, device=device) if top else None
+
+    def pointers(self):
+        return (self.logp.data_ptr(), self.entropy.data_ptr(), self.lse.data_ptr(), _raw(self.stats), _raw(self.top_logp), _raw(self.top_index))
+
+
+def log_probs(logits, targets, weights=None, scale=1.0, top=0, want_stats=True):
+    """logits [S,V], targets [S] i64, weights None / [V] / [S,V] f32 -> _Probs."""
     lib = _lib.load()
     S, V = logits.shape
     logits, ld = rows_2d(logits, V)
     weights, ldw = _row_weights(weights, V)
     targets = targets.contiguous()
     dev = logits.device
-    out, stats, top_logp, top_index = _log_probs_outputs(S, top, dev)
-    with torch.cuda.device(dev):
+    out = _Probs(S, top, want_stats, dev)
+    with _on(dev):
         nbytes = lib.nemo_log_probs_workspace(S, V, top)
         ws = _scratch(nbytes, dev)
-        check(lib.nemo_log_probs(_raw(logits), ld, _raw(weights), ldw, _raw(targets), S, V, DTYPES[logits.dtype], float(scale), int(top),
-                                 _raw(out[0]), _raw(out[1]), _raw(out[2]), _raw(stats), _raw(top_logp), _raw(top_index), _raw(ws), nbytes,
-                                 stream_ptr()), "nemo_log_probs")
-    return out, stats, top_logp, top_index
+        check(lib.nemo_log_probs(logits.data_ptr(), ld, _raw(weights), ldw, targets.data_ptr(), S, V, DTYPES[logits.dtype], scale, top,
+                                 *out.pointers(), _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_log_probs")
+    return out
 
 
 def log_probs_backward(logits, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0):
-    """-> grad_logits [S,V] in the type of the logits; the gradients are [S] f32 or None."""
+    """-> grad_logits [S,V] in the type of the logits; the gradients are [S] or None."""
     lib = _lib.load()
     S, V = logits.shape
     logits, ld = rows_2d(logits, V)
     weights, ldw = _row_weights(weights, V)
     targets = targets.contiguous()
-    gs = [None if g is None else g.detach().to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_lse)]
-    grad = torch.empty(S, V, dtype=logits.dtype, device=logits.device)
-    with torch.cuda.device(logits.device):
-        check(lib.nemo_log_probs_backward(_raw(logits), ld, _raw(weights), ldw, _raw(targets), _raw(stats), *[_raw(g) for g in gs], S, V,
-                                          DTYPES[logits.dtype], float(scale), _raw(grad), stream_ptr()), "nemo_log_probs_backward")
+    gs = [_f32_row(g) for g in (g_logp, g_entropy, g_lse)]
+    dev = logits.device
+    grad = torch.empty((S, V), dtype=logits.dtype, device=dev)
+    with _on(dev):
+        check(lib.nemo_log_probs_backward(logits.data_ptr(), ld, _raw(weights), ldw, targets.data_ptr(), stats.data_ptr(),
+                                          *[_raw(g) for g in gs], S, V, DTYPES[logits.dtype], scale, grad.data_ptr(), _raw_stream(dev.index)),
+              "nemo_log_probs_backward")
     return grad
 
 
-def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
+def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0, want_stats=True):
     """log_probs of scale features bank^T - weights without that matrix: features [S,C], bank [V,C] of one type.  Returns as log_probs."""
     lib = _lib.load()
     (S, ch), V = features.shape, bank.shape[0]
@@ -821,14 +844,14 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
     weights, ldw = _row_weights(weights, V)
     targets = targets.contiguous()
     dev, dt = features.device, DTYPES[features.dtype]
-    out, stats, top_logp, top_index = _log_probs_outputs(S, top, dev)
-    with torch.cuda.device(dev):
-        nbytes = lib.nemo_bank_log_probs_workspace(_raw(features), ldf, _raw(bank), ldb, S, V, ch, dt, top)
+    out = _Probs(S, top, want_stats, dev)
+    pf, pb = features.data_ptr(), bank.data_ptr()
+    with _on(dev):
+        nbytes = lib.nemo_bank_log_probs_workspace(pf, ldf, pb, ldb, S, V, ch, dt, top)
         ws = _scratch(nbytes, dev)
-        check(lib.nemo_bank_log_probs(_raw(features), ldf, _raw(bank), ldb, _raw(weights), ldw, _raw(targets), S, V, ch, dt, float(scale),
-                                      int(top), _raw(out[0]), _raw(out[1]), _raw(out[2]), _raw(stats), _raw(top_logp), _raw(top_index),
-                                      _raw(ws), nbytes, stream_ptr()), "nemo_bank_log_probs")
-    return out, stats, top_logp, top_index
+        check(lib.nemo_bank_log_probs(pf, ldf, pb, ldb, _raw(weights), ldw, targets.data_ptr(), S, V, ch, dt, scale, top, *out.pointers(),
+                                      _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_bank_log_probs")
+    return out
 
 
 def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_entropy, g_lse, scale=1.0, top=0, want=(True, True)):
@@ -840,13 +863,14 @@ def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_e
     weights, ldw = _row_weights(weights, V)
     targets = targets.contiguous()
     dev, dt = features.device, DTYPES[features.dtype]
-    gs = [None if g is None else g.detach().to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_lse)]
+    gs = [_f32_row(g) for g in (g_logp, g_entropy, g_lse)]
     empty = torch.zeros if S == 0 or V == 0 else torch.empty
-    grads = [empty(n, ch, dtype=features.dtype, device=dev) if w else None for n, w in zip((S, V), want)]
-    with torch.cuda.device(dev):
-        nbytes = lib.nemo_bank_log_probs_backward_workspace(_raw(features), ldf, _raw(bank), ldb, S, V, ch, dt)
+    grads = [empty((n, ch), dtype=features.dtype, device=dev) if w else None for n, w in zip((S, V), want)]
+    pf, pb = features.data_ptr(), bank.data_ptr()
+    with _on(dev):
+        nbytes = lib.nemo_bank_log_probs_backward_workspace(pf, ldf, pb, ldb, S, V, ch, dt)
         ws = _scratch(nbytes, dev)
-        check(lib.nemo_bank_log_probs_backward(_raw(features), ldf, _raw(bank), ldb, _raw(weights), ldw, _raw(targets), _raw(stats),
-                                               *[_raw(g) for g in gs], S, V, ch, dt, float(scale), int(top), *[_raw(g) for g in grads], _raw(ws),
-                                               nbytes, stream_ptr()), "nemo_bank_log_probs_backward")
+        check(lib.nemo_bank_log_probs_backward(pf, ldf, pb, ldb, _raw(weights), ldw, targets.data_ptr(), stats.data_ptr(),
+                                               *[_raw(g) for g in gs], S, V, ch, dt, scale, top, *[_raw(g) for g in grads], _raw(ws), nbytes,
+                                               _raw_stream(dev.index)), "nemo_bank_log_probs_backward")
     return tuple(grads)
