@@ -19,6 +19,7 @@
 // into the workspace with padded rows (pack_kernel).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/nemo_hip.h"
@@ -84,7 +85,7 @@ struct GemmArgs {
     const void* Q;
     long ldp, ldq;             // elements
     int np, nq, nk;
-    int big, tiles_p, tiles_q, splits, k_split;    // side of a tile; k of one split, whole steps
+    int bp, bq, tiles_p, tiles_q, splits, k_split; // sides of a tile; k of one split, whole steps
     float* partial;            // [splits][nq][np4] when splits > 1
     int np4;
     Epilogue e;
@@ -215,7 +216,7 @@ __device__ inline u32x4 fragment(const char* lds, int row, int kf, int lane) {
 // buffer; behind it, while the second half is multiplied, the tile after the next one is copied into that buffer and the first half of the
 // next tile is read.  So the matrix cores have work across the barrier, and a copy has a whole step to arrive.
 template <typename T, int BP, int BQ, int WP, int WQ, bool PT, bool QT>
-__global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 : 2) void gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 1 : BQ == 128 ? 2 : BQ == 64 ? 3 : 4) void gemm_kernel(GemmArgs a) {
     typedef Mma<T> M;
     constexpr int WAVES = WP * WQ, TP = BP / WP, TQ = BQ / WQ, NP = TP / M::FR, NQ = TQ / M::FR;
     constexpr int BK = kstep<T>(), HALF = BK / M::KF / 2;               // fragments of k in half a tile
@@ -307,10 +308,11 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
 
     // Through LDS into rows: a wave writes its results there (f32, in the buffers that held the tiles) and takes them back E consecutive columns
     // a lane, so that a row goes to memory in one piece, whatever its start, and the code that finishes a value stands here once.  Chunk c
-    // (16 bytes) of row r lies at c ^ (r & 15).
+    // (16 bytes) of row r lies at c ^ (r & FLIP).
+    constexpr int FLIP = TP / 4 < 16 ? TP / 4 - 1 : 15;
     constexpr int E = 16 / (int)sizeof(T), REGION = (BP + BQ) * 256 / WAVES, ROWS = REGION / (TP * 4), PASSES = TQ / ROWS > 0 ? TQ / ROWS : 1;
-    constexpr int FRAGS = NQ / PASSES, LANES = TP / E, ITERS = FRAGS * M::FR * LANES / 64, BATCH = 4;
-    static_assert(FRAGS * M::FR * TP * 4 <= REGION && TP / 4 >= 16 && ITERS % BATCH == 0, "a pass fits the wave's share of LDS");
+    constexpr int FRAGS = NQ / PASSES, LANES = TP / E, ITERS = FRAGS * M::FR * LANES / 64, BATCH = ITERS < 4 ? ITERS : 4;
+    static_assert(FRAGS * M::FR * TP * 4 <= REGION && ITERS % BATCH == 0, "a pass fits the wave's share of LDS");
     char* region = (wave < WAVES / 2 ? lds0 : lds1) + wave % (WAVES / 2) * REGION;
     const T* bias = (const T*)a.e.bias;
     const T* res = (const T*)a.e.residual;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
                 for (int b = 0; b < M::QUADS; ++b) {
                     const typename M::Acc& v = acc[i][pass * FRAGS + j];
                     const int r = j * M::FR + (lane & (M::FR - 1)), c = (i * M::FR + b * 8 + 4 * (lane / M::FR)) / 4;
-                    *(f32x4*)(region + r * (TP * 4) + ((c ^ (r & 15)) << 4)) = (f32x4){v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
+                    *(f32x4*)(region + r * (TP * 4) + ((c ^ (r & FLIP)) << 4)) = (f32x4){v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
                 }
         __syncthreads();
 #pragma unroll 1
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
                 float v[E];
 #pragma unroll
                 for (int k = 0; k < E / 4; ++k) {
-                    const f32x4 t = *(const f32x4*)(region + r * (TP * 4) + (((c0 / 4 + k) ^ (r & 15)) << 4));
+                    const f32x4 t = *(const f32x4*)(region + r * (TP * 4) + (((c0 / 4 + k) ^ (r & FLIP)) << 4));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[4 * k + i] = t[i];
                 }
@@ -384,11 +386,12 @@ __global__ __launch_bounds__(64 * WP * WQ, BP * BQ / (WP * WQ) >= 128 * 128 ? 1 
 // Sums the splits in their order and applies the epilogue; four columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
-    const int quads = a.np4 >> 2;
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long)quads * a.nq) return;
-    const int q = (int)(id / quads), p = 4 * (int)(id % quads);
+    const uint32_t quads = a.np4 >> 2, id = blockIdx.x * 256u + threadIdx.x;       // splits are of less than 256 tiles
+    if (id >= quads * (uint32_t)a.nq) return;
+    const uint32_t row = id / quads;
+    const int q = (int)row, p = 4 * (int)(id - row * quads);
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const f32x4 t = *(const f32x4*)(a.partial + ((size_t)s * a.nq + q) * a.np4 + p);
 #pragma unroll
@@ -397,31 +400,35 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
     epilogue_tail<T>(a.e, v, q, p, a.np);
 }
 
-// rows x cols (row stride ld, any start) -> rows x ld_out on 16 bytes, the columns beyond cols zero; 16 bytes of the copy a thread.
+// Copies with padded rows of one or two matrices: rows x cols (row stride ld, any start) -> rows x ld_out on 16 bytes, the columns beyond cols
+// zero; 16 bytes of the copy a thread.  The first `groups` workgroups take the first matrix.
+struct PackJob { const void* src; long ld; uint32_t rows; int cols; void* dst; int ld_out; };
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* src, long ld, long rows, int cols, T* dst, int ld_out) {
+__global__ __launch_bounds__(256) void pack_kernel(PackJob first, PackJob second, uint32_t groups) {
     constexpr int E = 16 / (int)sizeof(T);
-    const uint32_t per_row = ld_out / E;
-    const uint32_t id = blockIdx.x * 256u + threadIdx.x;                // fewer than 2^32 threads: see check_linear
+    const bool other = blockIdx.x >= groups;
+    const PackJob j = other ? second : first;
+    const uint32_t per_row = j.ld_out / E;
+    const uint32_t id = (blockIdx.x - (other ? groups : 0)) * 256u + threadIdx.x;
     const uint32_t r = id / per_row;
-    if (r >= rows) return;
+    if (r >= j.rows) return;
     const int c = (int)(id - r * per_row) * E;
-    const T* s = src + (long)r * ld + c;
+    const T* s = (const T*)j.src + (long)r * j.ld + c;
     typename Loose<T, E>::V v = {};
-    if (c + E <= cols) {
+    if (c + E <= j.cols) {
         v = load_loose<E>(s);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)
-            if (c + i < cols) v[i] = s[i];
+            if (c + i < j.cols) v[i] = s[i];
     }
-    *(typename Loose<T, E>::V*)(dst + (long)r * ld_out + c) = v;
+    *(typename Loose<T, E>::V*)((T*)j.dst + (long)r * j.ld_out + c) = v;
 }
 
 // dz = dy act'(pre) (rounded to T because the matrix cores take T), dr = beta dy, and per block of rows the column sums of the unrounded
 // dz (for the bias).  A workgroup takes 256 columns x ROWS rows: 32 threads of eight columns, eight rows at a time.  Bound by memory; rows
 // may start at any element.
-constexpr int kSlopeRows = 64;
+constexpr int kSlopeRows = 32;
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long ldg, const T* pre, long ldpre, long m, int n, int act, float beta,
                                                     T* dz, int ldz, T* dr, float* col_partial, int np4) {
@@ -486,6 +493,7 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float* partial, i
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     float t = 0.0f;
     if (c < n)
+#pragma unroll 4
         for (int b = part; b < blocks; b += 8) t += partial[(size_t)b * np4 + c];
     __shared__ float s[8][32];
     s[part][threadIdx.x & 31] = t;
@@ -505,19 +513,31 @@ static bool ready(const void* p, int64_t ld, int64_t cols, int es) {
     return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && (cols * es) % 16 == 0;
 }
 
-// Tiles of 256 x 256 (16-bit types, both operands plain, eight waves) where there are enough of them for every compute unit, else of 128 x 128 (four
-// waves).  8192 x 4096 x 4096 bf16: 218 us against 315 (128 x 128).  The addresses of transposed fragments take too many registers for the
-// large tile (460 us, against 313 with the small one).  Splits of k
-// for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least four steps of k.
-struct Shape { int big, tiles_p, tiles_q, splits, k_split; };
+// Tiles of 256 x 256 (16-bit types, both operands plain, eight waves) where there are enough of them for every compute unit; else four waves on
+// 128 columns x 128, 64 or 32 rows: fewer rows where there are no more, or where that gives no more than three tiles a unit and the sum is too
+// short to be split (up to 32 steps).  The addresses of transposed fragments take too many registers for the largest tile.  Measured in us (128 x 128 / 128 x 64 / 128 x 32):
+//     both transposed (a weight's gradient), f16, 515 x 1001 x 8191, split: 22 / 24 / 32
+//     f32   20 x 3678 x 128    15.5 / 11.0 /  7.4        bf16  20 x 3678 x 128      8.9 /  8.0 /  6.5
+//           1000 x 1000 x 1000 39.4 / 34.8 / 26.6              1000 x 1000 x 1000  20.7 / 20.7 / 10.3
+//           2000 x 2000 x 2048  145 /  140 /  145              2000 x 2000 x 2048  29.6 / 26.5 / 33.2
+//           8192 x 1024 x 2048  262 /  269 /  281              8192 x 1024 x 2048  39.1 / 45.5 / 59.3
+//     and 8192 x 4096 x 4096 bf16 218 with 256 x 256, 315 with 128 x 128.  f32 sums over at most 256 k leave so little to multiply in a tile
+//     that three workgroups a unit hide more of its ends: 5590 x 15976 x 128 with a residual 297 / 278 / 288.
+// Splits of k for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least four
+// steps of k.
+struct Shape { int bp, bq, tiles_p, tiles_q, splits, k_split; };
 static Shape shape_of(int64_t np, int64_t nq, int64_t nk, int dtype, bool transposed) {
     Shape s;
     const int step = 128 / elem_size(dtype);
-    s.big = dtype != NEMO_F32 && !transposed && np > 192 && nq > 192 && ((np + 255) / 256) * ((nq + 255) / 256) >= 240 ? 256 : 128;
-    s.tiles_p = (int)((np + s.big - 1) / s.big);
-    s.tiles_q = (int)((nq + s.big - 1) / s.big);
-    const int64_t tiles = (int64_t)s.tiles_p * s.tiles_q, steps = (nk + step - 1) / step;
-    int64_t want = tiles >= 256 || s.big == 256 ? 1 : 512 / tiles;
+    const bool big = dtype != NEMO_F32 && !transposed && np > 192 && nq > 192 && ((np + 255) / 256) * ((nq + 255) / 256) >= 240;
+    s.bp = big ? 256 : 128;
+    s.tiles_p = (int)((np + s.bp - 1) / s.bp);
+    const int64_t steps = (nk + step - 1) / step;
+    auto few = [&](int bq) { return nq <= bq || (steps <= 32 && s.tiles_p * ((nq + bq - 1) / bq) <= 3 * 256); };
+    s.bq = big ? 256 : few(32) ? 32 : few(64) || (dtype == NEMO_F32 && nk <= 256) ? 64 : 128;
+    s.tiles_q = (int)((nq + s.bq - 1) / s.bq);
+    const int64_t tiles = (int64_t)s.tiles_p * s.tiles_q;
+    int64_t want = tiles >= 256 || big ? 1 : 512 / tiles;
     if (want > steps / 4) want = steps / 4;
     if (want < 1) want = 1;
     const int64_t per = steps > 0 ? (steps + want - 1) / want : 1;
@@ -532,10 +552,14 @@ static size_t partial_bytes(int64_t np, int64_t nq, const Shape& s) {
 template <typename T, bool PT, bool QT>
 static void launch_gemm_typed(const GemmArgs& a, hipStream_t st) {
     const long wgs = (long)a.tiles_p * a.tiles_q * a.splits;
-    if (a.big == 256) {
+    if (a.bp == 256) {
         if constexpr (sizeof(T) == 2 && !PT) hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, PT, QT>), dim3((unsigned)wgs), dim3(512), 0, st, a);
-    } else {
+    } else if (a.bq == 128) {
         hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    } else if (a.bq == 64) {
+        hipLaunchKernelGGL((gemm_kernel<T, 128, 64, 2, 2, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((gemm_kernel<T, 128, 32, 4, 1, PT, QT>), dim3((unsigned)wgs), dim3(256), 0, st, a);
     }
     if (a.splits > 1) {
         const long threads = (long)(a.np4 / 4) * a.nq;
@@ -557,31 +581,52 @@ static void launch_gemm(int dtype, const GemmArgs& a, bool pt, bool qt, hipStrea
 }
 
 template <typename T>
-static void launch_pack(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int ld_out, hipStream_t st) {
-    const long threads = rows * (ld_out / (16 / (long)sizeof(T)));
-    hipLaunchKernelGGL((pack_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, (const T*)src, ld, rows, (int)cols, (T*)dst,
-                       ld_out);
+static void launch_pack(const PackJob* jobs, int n, hipStream_t st) {
+    int64_t groups[2] = {0, 0};
+    for (int i = 0; i < n; ++i) groups[i] = ((int64_t)jobs[i].rows * (jobs[i].ld_out / (16 / (int)sizeof(T))) + 255) / 256;
+    if (groups[0] + groups[1] <= 1 << 23) {
+        hipLaunchKernelGGL((pack_kernel<T>), dim3((unsigned)(groups[0] + groups[1])), dim3(256), 0, st, jobs[0], jobs[n - 1], (uint32_t)groups[0]);
+        return;
+    }
+    for (int i = 0; i < n; ++i) {                                      // a launch holds 2^32 threads: in slices of rows
+        const int64_t slice = (1LL << 31) / (jobs[i].ld_out / (16 / (int)sizeof(T)));
+        for (int64_t r = 0; r < jobs[i].rows; r += slice) {
+            PackJob j = jobs[i];
+            j.rows = (uint32_t)std::min<int64_t>(slice, jobs[i].rows - r);
+            j.src = (const T*)j.src + r * j.ld;
+            j.dst = (T*)j.dst + r * j.ld_out;
+            const unsigned wgs = (unsigned)(((int64_t)j.rows * (j.ld_out / (16 / (int)sizeof(T))) + 255) / 256);
+            hipLaunchKernelGGL((pack_kernel<T>), dim3(wgs), dim3(256), 0, st, j, j, wgs);
+        }
+    }
 }
 
-// An operand as the tiles want it: where it lies, or its packed copy taken from the workspace.
+// Operands as the tiles want them: where they lie, or packed copies taken from the workspace, made in one launch.
 struct Operand { const void* p; int64_t ld; };
-static Operand operand(int dtype, const void* p, int64_t ld, int64_t rows, int64_t cols, char*& ws, hipStream_t st) {
-    const int es = elem_size(dtype);
-    if (ready(p, ld, cols, es)) return {p, ld};
-    const int ld_out = pad16(cols, es);
-    void* dst = ws;
-    ws += align256((size_t)rows * ld_out * es);
-    if (dtype == NEMO_F32) launch_pack<float>(p, ld, rows, cols, dst, ld_out, st);
-    else if (dtype == NEMO_BF16) launch_pack<bf16>(p, ld, rows, cols, dst, ld_out, st);
-    else launch_pack<f16>(p, ld, rows, cols, dst, ld_out, st);
-    return {dst, ld_out};
-}
+struct Packer {
+    int dtype, n = 0;
+    PackJob jobs[2];
+    Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, char*& ws) {
+        const int es = elem_size(dtype);
+        if (rows == 0 || ready(p, ld, cols, es)) return {p, ld};
+        const int ld_out = pad16(cols, es);
+        void* dst = ws;
+        ws += align256((size_t)rows * ld_out * es);
+        jobs[n++] = {p, (long)ld, (uint32_t)rows, (int)cols, dst, ld_out};
+        return {dst, ld_out};
+    }
+    void launch(hipStream_t st) const {
+        if (n == 0) return;
+        if (dtype == NEMO_F32) launch_pack<float>(jobs, n, st);
+        else launch_pack<bf16>(jobs, n, st);                           // bits of either 16-bit type
+    }
+};
 
 static GemmArgs gemm_args(Operand P, Operand Q, int64_t np, int64_t nq, int64_t nk, const Shape& s, void* partial) {
     GemmArgs a = {};
     a.P = P.p; a.Q = Q.p; a.ldp = P.ld; a.ldq = Q.ld;
     a.np = (int)np; a.nq = (int)nq; a.nk = (int)nk;
-    a.big = s.big; a.tiles_p = s.tiles_p; a.tiles_q = s.tiles_q; a.splits = s.splits; a.k_split = s.k_split;
+    a.bp = s.bp; a.bq = s.bq; a.tiles_p = s.tiles_p; a.tiles_q = s.tiles_q; a.splits = s.splits; a.k_split = s.k_split;
     a.partial = (float*)partial;
     a.np4 = (int)((np + 3) / 4 * 4);
     a.e.alpha = 1.0f;
@@ -598,7 +643,7 @@ static int check_linear(const char* who, int64_t M, int64_t N, int64_t K, int dt
     if (M < 0 || N < 0 || K < 0) return fail(NEMO_ERR_INVALID, "%s: negative size", who);
     if (dtype != NEMO_F32 && dtype != NEMO_BF16 && dtype != NEMO_F16) return fail(NEMO_ERR_INVALID, "%s: unknown element type %d", who, dtype);
     if (act < 0 || act > 3) return fail(NEMO_ERR_INVALID, "%s: unknown activation %d", who, act);
-    // a launch holds 2^32 threads: 16 bytes of a copy a thread, a tile of 64 x 64 results a workgroup of 256
+    // a launch holds 2^32 threads: at least 64 x 64 results a workgroup of 256
     const int64_t pairs[3][2] = {{M, N}, {M, K}, {N, K}};
     for (const auto& p : pairs)
         if (p[0] > 0x7FFFF000 || p[1] > 0x7FFFF000 || p[0] * p[1] > (1LL << 34) || ((p[0] + 63) / 64) * ((p[1] + 63) / 64) > (1LL << 23))
@@ -637,12 +682,13 @@ extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
-    const int es = elem_size(dtype);
     char* ws = (char*)workspace;
     Operand P = {weight, ldw}, Q = {x, ldx};
     if (K > 0) {
-        P = operand(dtype, weight, ldw, N, K, ws, st);
-        Q = operand(dtype, x, ldx, M, K, ws, st);
+        Packer pack = {dtype};
+        P = pack.operand(weight, ldw, N, K, ws);
+        Q = pack.operand(x, ldx, M, K, ws);
+        pack.launch(st);
     }
     const Shape s = shape_of(N, M, K, dtype, false);
     GemmArgs a = gemm_args(P, Q, N, M, K, s, ws);
@@ -730,19 +776,24 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
         else
             launch_slope<f16>(grad_y, ldg, pre, M, N, activation, beta, dz_out, ldz, grad_residual, col_partial, grad_bias, st);
     }
+    Operand W = {weight, ldw}, X = {x, ldx};
+    if (K > 0) {
+        Packer pack = {dtype};
+        if (grad_x && M > 0) W = pack.operand(weight, ldw, N, K, ws);
+        if (grad_weight && N > 0) X = pack.operand(x, ldx, M, K, ws);
+        pack.launch(st);
+    }
     if (grad_x && M > 0 && K > 0) {
-        Operand W = N > 0 ? operand(dtype, weight, ldw, N, K, ws, st) : Operand{weight, ldw};
         const Shape s = shape_of(K, M, N, dtype, true);
         GemmArgs a = gemm_args(W, dz, K, M, N, s, ws);
         a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_x, K, nullptr};
-            launch_gemm(dtype, a, true, false, st);
+        launch_gemm(dtype, a, true, false, st);
     }
     if (grad_weight && N > 0 && K > 0) {
-        Operand X = M > 0 ? operand(dtype, x, ldx, M, K, ws, st) : Operand{x, ldx};
         const Shape s = shape_of(K, N, M, dtype, true);
         GemmArgs a = gemm_args(X, dz, K, N, M, s, ws);
         a.e = {alpha, 0.0f, ACT_NONE, nullptr, nullptr, 0, grad_weight, K, nullptr};
-            launch_gemm(dtype, a, true, true, st);
+        launch_gemm(dtype, a, true, true, st);
     }
     HIP_TRY(hipGetLastError());
     return NEMO_OK;
