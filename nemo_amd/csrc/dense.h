@@ -79,15 +79,32 @@ __device__ inline void copy_words_to_lds(const void* g, void* lds) {
 }
 
 // ---- reductions -----------------------------------------------------------------------------------------------------------------
+// Over the 64 lanes of a wave, all of them active, with the lane permutations of the vector units (a tenth of the latency of exchanges through
+// LDS): within four, eight and sixteen lanes, then lane 15 of a row of sixteen into the next one, lane 31 into the upper half; lane 63 has it all.
+template <int CTRL, int ROWS = 0xF> __device__ inline int permuted(int v, int other_rows) {
+    return __builtin_amdgcn_update_dpp(other_rows, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS = 0xF> __device__ inline float permuted(float v, float other_rows) {
+    return __builtin_bit_cast(float, permuted<CTRL, ROWS>(__builtin_bit_cast(int, v), __builtin_bit_cast(int, other_rows)));
+}
+template <typename V, typename Op> __device__ inline V wave_reduce(V v, V neutral, Op op) {
+    v = op(v, permuted<0xB1>(v, neutral));                             // lanes 1 0 3 2
+    v = op(v, permuted<0x4E>(v, neutral));                             // lanes 2 3 0 1
+    v = op(v, permuted<0x141>(v, neutral));                            // eight lanes mirrored
+    v = op(v, permuted<0x140>(v, neutral));                            // sixteen lanes mirrored
+    v = op(v, permuted<0x142, 0xA>(v, neutral));
+    v = op(v, permuted<0x143, 0xC>(v, neutral));
+    const int last = __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63);
+    return __builtin_bit_cast(V, last);
+}
 __device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
 __device__ inline float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return wave_reduce(v, neg_inf(), [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline int wave_min(int v) {
+    return wave_reduce(v, 0x7FFFFFFF, [](int a, int b) { return min(a, b); });
 }
 
 }  // namespace nemo

@@ -13,6 +13,9 @@
 #include "softmax_state.h"
 
 namespace nemo {
+#ifndef NEMO_U
+#define NEMO_U 4
+#endif
 
 struct LogProbArgs {
     const void* logits;
@@ -30,31 +33,32 @@ struct LogProbArgs {
     RowOut out;
 };
 
-template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T); T v[N]; };
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) LooseChunk { u32x4 v; };
+template <typename T> struct Chunk {
+    static constexpr int N = 16 / (int)sizeof(T);
+    typename Loose<T, N>::V v;
+    f32x4 w[N / 4];
+    // Logits and weights (w null: none) of N places from column j on, all of which exist.
+    __device__ inline void load(const T* row, const float* weights, int j) {
+        v = load_loose<N>(row + j);
+        if (weights) {
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) w[q] = load_loose<4>(weights + j + 4 * q);
+        }
+    }
+    __device__ inline void scores(bool weighted, float scale, float* z) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = weighted ? score(to_f32(v[i]), scale, w[i / 4][i % 4]) : score(to_f32(v[i]), scale);
+    }
+};
 
 // Scores of up to N places from column j on; places at or beyond `end` are -inf.
 template <typename T>
 __device__ inline void chunk_scores(const T* row, const float* w, float scale, int j, int end, float z[Chunk<T>::N]) {
     constexpr int N = Chunk<T>::N;
     if (j + N <= end) {
-        union { u32x4 u; T t[N]; } c;
-        c.u = ((const LooseChunk<T>*)(row + j))->v;
-        if (w) {
-            float wv[N];
-#pragma unroll
-            for (int q = 0; q < N / 4; ++q) {
-                const u32x4 u = ((const LooseChunk<float>*)(w + j + 4 * q))->v;
-                const f32x4 f = __builtin_bit_cast(f32x4, u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) wv[4 * q + i] = f[i];
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = score(to_f32(c.t[i]), scale, wv[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[i] = score(to_f32(c.t[i]), scale);
-        }
+        Chunk<T> c;
+        c.load(row, w, j);
+        c.scores(w != nullptr, scale, z);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -62,9 +66,9 @@ __device__ inline void chunk_scores(const T* row, const float* w, float scale, i
     }
 }
 
-// A chunk's scores into a state: one rescaling a chunk.
+// N scores into a state: one rescaling for all of them.
 template <int N>
-__device__ inline void add_scores(SoftmaxState& a, const float z[N]) {
+__device__ inline void add_scores(SoftmaxState& a, const float* z) {
     float m = a.m;
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
@@ -80,7 +84,7 @@ __device__ inline void add_scores(SoftmaxState& a, const float z[N]) {
 // WAVES waves a row, ROWS rows a workgroup (WAVES * ROWS = 4).
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
-    constexpr int N = Chunk<T>::N, ROWS = 4 / WAVES, LANES = 64 * WAVES;
+    constexpr int N = Chunk<T>::N, ROWS = 4 / WAVES, LANES = 64 * WAVES, UNROLL = NEMO_U;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int part = (int)(blockIdx.x % a.parts);
     const long row = (long)(blockIdx.x / a.parts) * ROWS + wave / WAVES;
@@ -93,16 +97,29 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
     SoftmaxState st = empty_state();
     Entry best = no_entry();
     if (live) {
-#pragma unroll 2
-        for (int j = first; j < end; j += LANES * N) {
+        // places rise within a lane: the first of equal ones stays
+        auto keep = [&](float z, int place) __attribute__((always_inline)) {
+            if (TOP && z > best.z) best = {z, place};
+        };
+        // UNROLL loads under way at once
+        int j = first;
+        for (; j + (UNROLL - 1) * LANES * N + N <= end; j += UNROLL * LANES * N) {
+            Chunk<T> c[UNROLL];
+            float z[UNROLL * N];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) c[u].load(logits, w, j + u * LANES * N);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) c[u].scores(w != nullptr, a.scale, z + u * N);
+            add_scores<UNROLL * N>(st, z);
+#pragma unroll
+            for (int i = 0; i < UNROLL * N; ++i) keep(z[i], j + i / N * (LANES * N) + i % N);
+        }
+        for (; j < end; j += LANES * N) {
             float z[N];
             chunk_scores<T>(logits, w, a.scale, j, end, z);
             add_scores<N>(st, z);
-            if (TOP) {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (z[i] > best.z) best = {z[i], j + i};           // places rise within a lane: the first of equal ones stays
-            }
+            for (int i = 0; i < N; ++i) keep(z[i], j + i);
         }
     }
     st = wave_join(st, kLog2e);
@@ -221,20 +238,20 @@ __global__ __launch_bounds__(256) void log_probs_backward_kernel(LogProbArgs a, 
         for (int j = (blockIdx.x * 256 + threadIdx.x) * N; j < a.cols; j += gridDim.x * 256 * N) {
             float z[N];
             chunk_scores<T>(logits, w, a.scale, j, a.cols, z);
-            union { u32x4 u; T t[N]; } c;
+            typename Loose<T, N>::V c;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float d = prob_gradient(__builtin_fmaf(z[i] - k.m, kLog2e, -k.log2_s), k.c, k.g2);
                 if (j + i == k.target) d += k.g_logp;
                 if (z[i] == neg_inf()) d = 0.0f;
-                c.t[i] = from_f32<T>(a.scale * d);
+                c[i] = from_f32<T>(a.scale * d);
             }
             if (j + N <= a.cols) {
-                ((LooseChunk<T>*)(out + j))->v = c.u;
+                store_loose<N>(out + j, c);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (j + i < a.cols) out[j + i] = c.t[i];
+                    if (j + i < a.cols) out[j + i] = c[i];
             }
         }
     }

@@ -36,21 +36,20 @@ __device__ inline SoftmaxState join_states(const SoftmaxState& a, const SoftmaxS
     return r;
 }
 
-__device__ inline SoftmaxState wave_join(SoftmaxState a, float unit) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const SoftmaxState b = {__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
-        a = join_states(a, b, unit);
-    }
-    return a;
-}
-
 // Makes room for scores up to `m`: the old sums in the new units.
 __device__ inline void raise(SoftmaxState& a, float m, float unit) {
     const float d = (a.m - m) * unit, f = exp2_fast(d);
     a.t = f * (a.t + fmaxf(d, -1.0e4f) * a.s);
     a.s *= f;
     a.m = m;
+}
+
+// The states of a wave's lanes as one, the same in every lane.
+__device__ inline SoftmaxState wave_join(SoftmaxState a, float unit) {
+    raise(a, wave_max(a.m), unit);
+    a.s = wave_sum(a.s);
+    a.t = wave_sum(a.t);
+    return a;
 }
 
 __device__ inline float score(float logit, float scale) { return __fmul_rn(logit, scale); }
@@ -62,17 +61,13 @@ __device__ inline float score(float logit, float scale, float w) {
 struct Entry { float z; int place; };
 __device__ inline bool ahead(const Entry& a, const Entry& b) { return a.z > b.z || (a.z == b.z && a.place < b.place); }
 
-__device__ inline Entry wave_best(Entry a) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const Entry b = {__shfl_xor(a.z, o), __shfl_xor(a.place, o)};
-        if (ahead(b, a)) a = b;
-    }
-    return a;
-}
-
 constexpr int kNoPlace = 0x7FFFFFFF;               // sorts behind every place of the same score
 __device__ inline Entry no_entry() { return {neg_inf(), kNoPlace}; }
+// The first of a wave's entries, the same in every lane.
+__device__ inline Entry wave_best(const Entry& a) {
+    const float z = wave_max(a.z);
+    return {z, wave_min(a.z == z ? a.place : kNoPlace)};
+}
 
 // What a call returns for a row, from its joined state.
 struct RowOut {
