@@ -7,15 +7,13 @@
 // Rows need not be aligned: 16-byte accesses at any element are in order on this hardware.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "../../include/nemo_hip.h"
 #include "errors.h"
 #include "softmax_state.h"
 
 namespace nemo {
-#ifndef NEMO_U
-#define NEMO_U 4
-#endif
 
 struct LogProbArgs {
     const void* logits;
@@ -37,32 +35,32 @@ template <typename T> struct Chunk {
     static constexpr int N = 16 / (int)sizeof(T);
     typename Loose<T, N>::V v;
     f32x4 w[N / 4];
-    // Logits and weights (w null: none) of N places from column j on, all of which exist.
-    __device__ inline void load(const T* row, const float* weights, int j) {
+    // Logits and, with W, weights of N places from column j on, all of which exist.
+    template <bool W> __device__ inline void load(const T* row, const float* weights, int j) {
         v = load_loose<N>(row + j);
-        if (weights) {
+        if (W) {
 #pragma unroll
             for (int q = 0; q < N / 4; ++q) w[q] = load_loose<4>(weights + j + 4 * q);
         }
     }
-    __device__ inline void scores(bool weighted, float scale, float* z) const {
+    template <bool W> __device__ inline void scores(float scale, float* z) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = weighted ? score(to_f32(v[i]), scale, w[i / 4][i % 4]) : score(to_f32(v[i]), scale);
+        for (int i = 0; i < N; ++i) z[i] = W ? score(to_f32(v[i]), scale, w[i / 4][i % 4]) : score(to_f32(v[i]), scale);
     }
 };
 
 // Scores of up to N places from column j on; places at or beyond `end` are -inf.
-template <typename T>
+template <bool W, typename T>
 __device__ inline void chunk_scores(const T* row, const float* w, float scale, int j, int end, float z[Chunk<T>::N]) {
     constexpr int N = Chunk<T>::N;
     if (j + N <= end) {
         Chunk<T> c;
-        c.load(row, w, j);
-        c.scores(w != nullptr, scale, z);
+        c.template load<W>(row, w, j);
+        c.template scores<W>(scale, z);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            z[i] = j + i >= end ? neg_inf() : w ? score(to_f32(row[j + i]), scale, w[j + i]) : score(to_f32(row[j + i]), scale);
+            z[i] = j + i >= end ? neg_inf() : W ? score(to_f32(row[j + i]), scale, w[j + i]) : score(to_f32(row[j + i]), scale);
     }
 }
 
@@ -81,10 +79,34 @@ __device__ inline void add_scores(SoftmaxState& a, const float* z) {
     }
 }
 
+// The same with fewer operations: x = fma(z, log2 e, -u) against the rounded u = m log2 e, which drops out when the state is turned into the
+// other form.  Scores beyond 1e38 and, without LEFT_OUT, scores of -inf make s 0 or s or t NaN; the wave then goes through its share again.
+struct QuickState {
+    float m = -1.0e38f, u = -1.0e38f * kLog2e, s = 0.0f, t = 0.0f;
+    template <int N, bool LEFT_OUT> __device__ inline void add(const float* z) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
+        const float up = m * kLog2e, d = u - up, f = exp2_fast(d);
+        t = f * (t + fmaxf(d, -1.0e4f) * s);
+        s *= f;
+        u = up;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float x = __builtin_fmaf(z[i], kLog2e, -u), e = exp2_fast(x);
+            s += e;
+            t += e * (LEFT_OUT ? fmaxf(x, -200.0f) : x);
+        }
+    }
+    __device__ inline SoftmaxState state() const {
+        const float d = -__builtin_fmaf(m, kLog2e, -u), f = exp2_fast(d);
+        return {m, s * f, f * (t + d * s)};
+    }
+};
+
 // WAVES waves a row, ROWS rows a workgroup (WAVES * ROWS = 4).
-template <typename T, int WAVES, bool TOP>
+template <typename T, int WAVES, bool TOP, bool W>
 __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
-    constexpr int N = Chunk<T>::N, ROWS = 4 / WAVES, LANES = 64 * WAVES, UNROLL = NEMO_U;
+    constexpr int N = Chunk<T>::N, ROWS = 4 / WAVES, LANES = 64 * WAVES, UNROLL = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int part = (int)(blockIdx.x % a.parts);
     const long row = (long)(blockIdx.x / a.parts) * ROWS + wave / WAVES;
@@ -92,9 +114,9 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
     const int wr = wave % WAVES;
     const int begin = part * a.part_cols, end = min(a.cols, begin + a.part_cols);
     const T* logits = (const T*)a.logits + (live ? row : 0) * a.ld;
-    const float* w = a.weights ? a.weights + (live ? row : 0) * a.ldw : nullptr;
+    const float* w = W ? a.weights + (live ? row : 0) * a.ldw : nullptr;
     const int first = begin + (wr * 64 + lane) * N;
-    SoftmaxState st = empty_state();
+    QuickState quick;
     Entry best = no_entry();
     if (live) {
         // places rise within a lane: the first of equal ones stays
@@ -107,22 +129,31 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
             Chunk<T> c[UNROLL];
             float z[UNROLL * N];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) c[u].load(logits, w, j + u * LANES * N);
+            for (int u = 0; u < UNROLL; ++u) c[u].template load<W>(logits, w, j + u * LANES * N);
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) c[u].scores(w != nullptr, a.scale, z + u * N);
-            add_scores<UNROLL * N>(st, z);
+            for (int u = 0; u < UNROLL; ++u) c[u].template scores<W>(a.scale, z + u * N);
+            quick.add<UNROLL * N, W>(z);
 #pragma unroll
             for (int i = 0; i < UNROLL * N; ++i) keep(z[i], j + i / N * (LANES * N) + i % N);
         }
         for (; j < end; j += LANES * N) {
             float z[N];
-            chunk_scores<T>(logits, w, a.scale, j, end, z);
-            add_scores<N>(st, z);
+            chunk_scores<W>(logits, w, a.scale, j, end, z);
+            quick.add<N, true>(z);
 #pragma unroll
             for (int i = 0; i < N; ++i) keep(z[i], j + i);
         }
     }
-    st = wave_join(st, kLog2e);
+    SoftmaxState st = wave_join(quick.state(), kLog2e);
+    if (live && !(st.s > 0.0f && st.t == st.t)) {                      // nothing counted, or a value that QuickState does not take
+        st = empty_state();
+        for (int j = first; j < end; j += LANES * N) {
+            float z[N];
+            chunk_scores<W>(logits, w, a.scale, j, end, z);
+            add_scores<N>(st, z);
+        }
+        st = wave_join(st, kLog2e);
+    }
     __shared__ SoftmaxState s_state[4];
     __shared__ Entry s_top[TOP ? 4 : 1][kMaxTop];
     const int top = a.out.top;
@@ -140,7 +171,7 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
             Entry next = no_entry();
             for (int j = begin + (wr * 64 + owner) * N + lane * LANES * N; j < end; j += 64 * LANES * N) {
                 float z[N];
-                chunk_scores<T>(logits, w, a.scale, j, end, z);
+                chunk_scores<W>(logits, w, a.scale, j, end, z);
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
                     const Entry c = {z[q], j + q};
@@ -173,7 +204,7 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
     } else if (lane == 0) {
         const long long t = a.targets[row];
         float zt = 0.0f;
-        if (t >= 0 && t < a.cols) zt = w ? score(to_f32(logits[t]), a.scale, w[t]) : score(to_f32(logits[t]), a.scale);
+        if (t >= 0 && t < a.cols) zt = W ? score(to_f32(logits[t]), a.scale, w[t]) : score(to_f32(logits[t]), a.scale);
         write_row(a.out, row, st, t, a.cols, zt);
     }
     if (TOP) {
@@ -225,19 +256,19 @@ __global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a) {
 }
 
 // d logits: 256 threads x 16 bytes a step of a row.
-template <typename T>
+template <typename T, bool W>
 __global__ __launch_bounds__(256) void log_probs_backward_kernel(LogProbArgs a, const float* stats, const float* g_logp, const float* g_entropy,
                                                                  const float* g_lse, T* grad) {
     constexpr int N = Chunk<T>::N;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const RowCoef k = row_coef(stats, g_logp, g_entropy, g_lse, a.targets, row, a.cols);
         const T* logits = (const T*)a.logits + row * a.ld;
-        const float* w = a.weights ? a.weights + row * a.ldw : nullptr;
+        const float* w = W ? a.weights + row * a.ldw : nullptr;
         T* out = grad + row * (long)a.cols;
 #pragma unroll 2
         for (int j = (blockIdx.x * 256 + threadIdx.x) * N; j < a.cols; j += gridDim.x * 256 * N) {
             float z[N];
-            chunk_scores<T>(logits, w, a.scale, j, a.cols, z);
+            chunk_scores<W>(logits, w, a.scale, j, a.cols, z);
             typename Loose<T, N>::V c;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -279,13 +310,15 @@ static void launch_log_probs(const LogProbArgs& a, hipStream_t st) {
     // One wave a row where a row is short and there are enough of them to fill the device that way; four waves a row otherwise.
     const bool narrow = a.cols <= 2048 && a.rows >= 2048;
     const unsigned wgs = narrow ? (unsigned)((a.rows + 3) / 4) : (unsigned)(a.rows * a.parts);
-    if (a.out.top) {
-        if (narrow) hipLaunchKernelGGL((log_probs_kernel<T, 1, true>), dim3(wgs), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((log_probs_kernel<T, 4, true>), dim3(wgs), dim3(256), 0, st, a);
-    } else {
-        if (narrow) hipLaunchKernelGGL((log_probs_kernel<T, 1, false>), dim3(wgs), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((log_probs_kernel<T, 4, false>), dim3(wgs), dim3(256), 0, st, a);
-    }
+    auto launch = [&](auto top, auto weighted) {
+        constexpr bool TOP = decltype(top)::value, W = decltype(weighted)::value;
+        if (narrow) hipLaunchKernelGGL((log_probs_kernel<T, 1, TOP, W>), dim3(wgs), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((log_probs_kernel<T, 4, TOP, W>), dim3(wgs), dim3(256), 0, st, a);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (a.out.top) a.weights ? launch(yes, yes) : launch(yes, no);
+    else a.weights ? launch(no, yes) : launch(no, no);
     if (a.parts > 1) hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
 }
 
@@ -339,8 +372,11 @@ static void launch_log_probs_backward(const LogProbArgs& a, const float* stats, 
                                       void* grad, hipStream_t st) {
     const int per = 256 * Chunk<T>::N;
     const int slabs = (a.cols + 2 * per - 1) / (2 * per);              // two steps a thread
-    hipLaunchKernelGGL((log_probs_backward_kernel<T>), dim3(slabs, (unsigned)(a.rows < 65535 ? a.rows : 65535)), dim3(256), 0, st, a, stats, g_logp,
-                       g_entropy, g_lse, (T*)grad);
+    const dim3 grid(slabs, (unsigned)(a.rows < 65535 ? a.rows : 65535));
+    if (a.weights)
+        hipLaunchKernelGGL((log_probs_backward_kernel<T, true>), grid, dim3(256), 0, st, a, stats, g_logp, g_entropy, g_lse, (T*)grad);
+    else
+        hipLaunchKernelGGL((log_probs_backward_kernel<T, false>), grid, dim3(256), 0, st, a, stats, g_logp, g_entropy, g_lse, (T*)grad);
 }
 
 extern "C" int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights, int64_t ldw, const int64_t* targets,
