@@ -473,9 +473,10 @@ int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights
 
 /* nemo_log_probs straight from features [rows,channels] and bank [cols,channels] (f32 or bf16, both the same):
  *   z[i,j] = scale <features[i], bank[j]> - weights[i,j],
- * same outputs and rules, the [rows,cols] matrix is never written.  Products are summed in f32 (f32: on the f32 matrix cores).  channels
- * 1..256 (padded to 64, 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same
- * pointers and strides (rows that do not start on 16 bytes are copied into it), contents undefined before and after. */
+ * same outputs and rules, the [rows,cols] matrix is never written.  Products are summed in f32.  f32 rows are multiplied as three bf16 pieces
+ * (24 bits together, as exact as f32 products; an infinity in a row makes its scores NaN, whatever its sign).  channels 1..256 (padded to 64,
+ * 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same pointers and strides
+ * (pieces, and rows that do not start on 16 bytes, are written into it), contents undefined before and after. */
 size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                      int64_t channels, int32_t dtype, int32_t top);
 int nemo_bank_log_probs(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,
@@ -486,7 +487,8 @@ int nemo_bank_log_probs(const void* features, int64_t ldf, const void* bank, int
  *   grad_features[i] = scale sum_j dz[i,j] bank[j],   grad_bank[j] = scale sum_i dz[i,j] features[i]
  * (contiguous, element type dtype; NULL: not wanted).  weights, scale and top as in the call that wrote `stats` (they decide the form in
  * which it is kept).  The scores are computed again.  Places that are left out add nothing, whatever the
- * feature or bank row holds.  Sums run in a fixed order: two calls give the same bits. */
+ * feature or bank row holds.  Rows whose target is outside -1..cols-1 make grad_features[i] and all of grad_bank NaN.  bf16: dz is
+ * multiplied as two bf16 pieces, f32: as three.  Sums run in a fixed order: two calls give the same bits. */
 size_t nemo_bank_log_probs_backward_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                               int64_t channels, int32_t dtype);
 int nemo_bank_log_probs_backward(const void* features, int64_t ldf, const void* bank, int64_t ldb, const float* weights, int64_t ldw,

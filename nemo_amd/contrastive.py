@@ -14,10 +14,10 @@ from . import ops
 
 
 def _device_tensors(what, dtypes, names, *tensors):
-    """All tensors on one GPU and of one of `dtypes` (None entries are skipped)."""
+    """All tensors on one GPU and of one of `dtypes`; bias and residual may be None."""
     first = tensors[0]
     for name, t in zip(names, tensors):
-        if t is None:
+        if t is None and name in ("bias", "residual"):
             continue
         if not torch.is_tensor(t):
             raise TypeError(f"{what}: {name} must be a tensor")
@@ -201,8 +201,10 @@ class _BankLogProbs(torch.autograd.Function):
 
 def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
     """log_probs(linear(features, bank), ...) without the [S, V] matrix: features [S, C] and bank [V, C], both float32 or both bfloat16, C up
-    to 256.  Scores are z = scale <feature, bank row> - weights, summed in 32 bits; arguments, results and rules are those of log_probs.
-    Differentiable with respect to features and bank; the gradient computes the scores again instead of keeping them."""
+    to 256, S and V below 2^24.  Scores are z = scale <feature, bank row> - weights, summed in 32 bits; arguments, results and rules are
+    those of log_probs.  float32 rows are multiplied as three bfloat16 pieces (24 bits together): products are as exact as float32's, but
+    an infinity in a row makes its scores NaN, whatever its sign.  Differentiable with respect to features and bank; the gradient computes
+    the scores again instead of keeping them; it may be split in another way than the values, and two calls give the same bits."""
     _device_tensors("bank_log_probs", (torch.float32, torch.bfloat16), ("features", "bank"), features, bank)
     if features.dim() != 2 or bank.dim() != 2 or features.shape[1] != bank.shape[1]:
         raise ValueError(f"bank_log_probs: features must be [S, C] and bank [V, C], got {tuple(features.shape)} and {tuple(bank.shape)}")

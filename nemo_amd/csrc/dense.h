@@ -1,5 +1,5 @@
-// What the dense operators (linear.hip, log_probs.hip, bank_log_probs.hip) share: element types, matrix-core fragments, the
-// direct copy from global memory to LDS, reductions.
+// What the dense operators (linear.hip, log_probs.hip, the bank kernels) share: element types, accesses at any element, the matrix-core fragments
+// of linear.hip, the direct copy from global memory to LDS, reductions over a wave.
 //
 // A fragment is 16 bytes a lane, for either operand of a product:
 //   16-bit types  v_mfma_f32_16x16x32: lane = (row r = lane % 16, group g = lane / 16), elements k = 8 g .. 8 g + 7 of a block of 32;

@@ -1,10 +1,15 @@
 // Log probabilities of given places of rows of logits, with entropy, log-sum-exp and the best entries; and the gradient of the logits.
 //
-// Both directions read each logit once and are bound by memory.  Forward: a wave or a workgroup of four waves takes a row (or one of its
-// parts), a lane takes 16 bytes at a time and keeps the state of softmax_state.h; states are joined across lanes, waves and parts in a
-// fixed order.  For the best entries a lane keeps its best one; a wave takes the best of its lanes k times, and the lane it came from
+// Both directions read each logit once.  Forward: a wave or a workgroup of four waves takes a row (or one of its parts), a lane takes 16 bytes
+// at a time, four of them under way at once, and keeps the state of softmax_state.h; states are joined across lanes, waves and parts in
+// a fixed order.  For the best entries a lane keeps its best one; a wave takes the best of its lanes k times, and the lane it came from
 // looks through its share of the row again for the next one, together with the whole wave.  Waves' lists, sorted, are merged.
 // Rows need not be aligned: 16-byte accesses at any element are in order on this hardware.
+//
+// Measured.  4096 x 100003 bf16 (819 MB): forward 213 us, 3.9 TB/s, the vector units 71 % busy (7.5 instructions a score, one of them the
+// exponential, four times as long); backward 352 us for as much read and written, 4.7 TB/s, what a copy reaches.  8000 x 13416 f32 with the five
+// best (429 MB): 91 us, 4.7 TB/s; with weights for every place, without a list (858 MB): 170 us, 5.1 TB/s.  One row of 1118 f32 with the five
+// best: 7.5 us, the latency of a launch, of a few dependent loads and of five selections.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
@@ -80,9 +85,10 @@ __device__ inline void add_scores(SoftmaxState& a, const float* z) {
 }
 
 // The same with fewer operations: x = fma(z, log2 e, -u) against the rounded u = m log2 e, which drops out when the state is turned into the
-// other form.  Scores beyond 1e38 and, without LEFT_OUT, scores of -inf make s 0 or s or t NaN; the wave then goes through its share again.
+// other form.  Scores beyond 2^126 and, without LEFT_OUT, scores of -inf make s 0 or s or t NaN; the wave then goes through its share again.
+// (4096 x 100003 bf16: 224 us with the other form, of which the vector units were busy 150; 8000 x 13416 f32 with a list 99 against 91.)
 struct QuickState {
-    float m = -1.0e38f, u = -1.0e38f * kLog2e, s = 0.0f, t = 0.0f;
+    float m = -0x1p126f, u = -0x1p126f * kLog2e, s = 0.0f, t = 0.0f;       // u exact: a lane without scores stays 0
     template <int N, bool LEFT_OUT> __device__ inline void add(const float* z) {
 #pragma unroll
         for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);

@@ -103,6 +103,14 @@ def test_linear_sizes(gpu, M, N, K, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,N,K", [(32, 300, 512), (33, 1000, 2100), (900, 50, 300), (5000, 700, 1030), (6000, 2000, 100), (7900, 2049, 70)])
+def test_linear_every_tile(gpu, M, N, K, dtype):
+    """Sizes for which the products of the three directions take tiles of 32, 64, 128 and 256 rows, with and without splits."""
+    linear_case(gpu, M, N, K, TYPES[dtype], "silu", residual=(M % 2 == 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("act", list(ACT))
 @pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True), (True, True)])
 def test_linear_epilogues(gpu, act, bias, residual, dtype):
@@ -431,6 +439,36 @@ def test_log_probs_rows_that_masks_leave(gpu, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("V", [300, 5000, 20001])
+def test_log_probs_extreme_scores(gpu, V, top):
+    """Without weights: masks of -inf and of the lowest value, scores up to the type's largest, infinities and NaN that count."""
+    import nemo_amd
+    gen = torch.Generator(device=gpu).manual_seed(V)
+    base, at = torch.randn(V, generator=gen, device=gpu), torch.arange(V, device=gpu)
+    full = lambda v: torch.full((V,), v, device=gpu)
+    low = -3.4028234663852886e38
+    rows = [base, full(-INF), torch.where(at < V - 7, -INF, base), torch.where(at % 2 == 0, -INF, base), full(low), torch.where(at < V - 7, low, base),
+            full(-2.0e38), torch.where(at == 9, 3.0e38, base), full(2.5e38), torch.where(at == 17, float("nan"), base), torch.where(at == V - 1, INF, base),
+            full(1.0e5), full(-1.0e5), 1.0e4 + 8 * torch.round(base), torch.where(at == 3, -1.0e38, full(-3.0e38))]
+    logits = torch.stack(rows)
+    S = len(rows)
+    targets = torch.full((S,), V - 3, device=gpu)
+    targets[1], targets[7], targets[14] = 5, 9, 3
+    g = upstream(S, gen, gpu)
+    leaf = logits.clone().requires_grad_()
+    r = nemo_amd.log_probs(leaf, targets, top=top)
+    z = logits.double()
+    ref = probs_reference(z, targets, top, g)
+    bounds = probs_bounds(ref, torch.where(z.abs() < 1e30, z, torch.zeros_like(z)), torch.zeros(S, device=gpu, dtype=torch.float64), V, g)
+    bounds["lse"] = bounds["lse"] + 4 * U * torch.where(torch.isfinite(ref["lse"]), ref["lse"].abs(), torch.zeros_like(ref["lse"]))
+    check_probs(r, ref, bounds, top)
+    (gx,) = run_grads(r, g, [leaf])
+    within(gx, ref["dz"], torch.nan_to_num(bounds["dz"] + U * (ref["dz"].abs() + bounds["dz"])), "gradient")
+    assert not gx[1].any()
+
+
+@pytest.mark.gpu
 def test_log_probs_empty_shapes(gpu):
     import nemo_amd
     for fn in (lambda S, V, top: nemo_amd.log_probs(torch.zeros(S, V, device=gpu), torch.full((S,), -1, device=gpu), top=top),
@@ -508,7 +546,8 @@ def bank_case(dev, S, V, ch, dtype, kind, top, scale=4.0, which="logp entropy ls
     raw = F @ Bk.T
     z = scores64(raw, scale, weights)
     ref = probs_reference(z, targets, top, g)
-    mag = scale * (torch.nan_to_num(F, 0, 0, 0).abs() @ torch.nan_to_num(Bk, 0, 0, 0).abs().T)
+    size = abs(scale)
+    mag = size * (torch.nan_to_num(F, 0, 0, 0).abs() @ torch.nan_to_num(Bk, 0, 0, 0).abs().T)
     live = ref["p"] > 1e-40
     fw = 0.0 if weights is None else torch.where(torch.isfinite(weights), weights, torch.zeros_like(weights)).double()
     z_err = torch.where(live, (ch + 4) * U * mag + 2 * U * (mag + fw), torch.zeros_like(z)).amax(1)
@@ -519,8 +558,8 @@ def bank_case(dev, S, V, ch, dtype, kind, top, scale=4.0, which="logp entropy ls
     Fc, Bc = torch.nan_to_num(F, 0, 0, 0), torch.nan_to_num(Bk, 0, 0, 0)          # what is left out adds nothing, whatever it holds
     piece = 0.0 if dtype == torch.float32 else 2.0 ** -16                          # two bf16 pieces of dz, 8 bits each
     dz, e = ref["dz"], bounds["dz"] + piece * ref["dz"].abs() + (0 if piece == 0 else 1e-38)
-    for name, got, want, err, n in (("features", gf, scale * dz @ Bc, scale * (e + (V + 4) * U * dz.abs()) @ Bc.abs(), V),
-                                    ("bank", gb, scale * dz.T @ Fc, scale * (e + (S + 4) * U * dz.abs()).T @ Fc.abs(), S)):
+    for name, got, want, err, n in (("features", gf, scale * dz @ Bc, size * (e + (V + 4) * U * dz.abs()) @ Bc.abs(), V),
+                                    ("bank", gb, scale * dz.T @ Fc, size * (e + (S + 4) * U * dz.abs()).T @ Fc.abs(), S)):
         within(got, want, torch.nan_to_num(err + half_step(dtype) * (want.abs() + err) + tiny(dtype)), f"gradient of {name}")
 
 
@@ -538,6 +577,45 @@ def test_bank_log_probs_sizes(gpu, S, V, ch, kind, dtype):
 @pytest.mark.parametrize("which", ["logp", "entropy", "lse"])
 def test_bank_log_probs_single_gradients(gpu, which):
     bank_case(gpu, 70, 200, 32, torch.float32, "rows", 0, which=which)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [-4.0, 0.0, 1e-35, 60.0])
+@pytest.mark.parametrize("kind", ["none", "rows"])
+def test_bank_log_probs_scales(gpu, kind, scale, dtype):
+    bank_case(gpu, 150, 333, 64, TYPES[dtype], kind, 0 if scale == 1e-35 else 5, scale=scale)
+    bank_case(gpu, 150, 333, 64, TYPES[dtype], kind, 0, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [300.0, -300.0])
+def test_bank_log_probs_scores_far_below_zero(gpu, scale, dtype):
+    """The zeros behind the last bank row, and behind the last feature row, must not count beside scores of -300."""
+    gen = torch.Generator(device=gpu).manual_seed(3)
+    u = torch.nn.functional.normalize(torch.randn(1, 100, generator=gen, device=gpu), dim=1)
+    near = lambda n: torch.nn.functional.normalize(u + 0.02 * torch.randn(n, 100, generator=gen, device=gpu), dim=1)
+    f, b = near(70).to(TYPES[dtype]), (near(333) * (-1.0 if scale > 0 else 1.0)).to(TYPES[dtype])
+    for kind in ("none", "rows"):
+        bank_case(gpu, 70, 333, 100, TYPES[dtype], kind, 0, scale=scale, features=f, bank=b)
+
+
+@pytest.mark.gpu
+def test_bank_log_probs_far_apart_magnitudes_and_repeated_targets(gpu):
+    """f32 rows as pieces: powers of two of the rows change no bit.  All slots share two targets."""
+    import nemo_amd
+    gen = torch.Generator(device=gpu).manual_seed(8)
+    f, b = torch.randn(100, 40, generator=gen, device=gpu), torch.randn(77, 40, generator=gen, device=gpu)
+    t = 13 * torch.randint(0, 2, (100,), generator=gen, device=gpu)
+    bank_case(gpu, 100, 77, 40, torch.float32, "none", 0, scale=0.5, features=f, bank=b, targets=t)
+    p, q = nemo_amd.bank_log_probs(f, b, t, scale=0.5, top=3), nemo_amd.bank_log_probs(f * 2.0 ** 60, b * 2.0 ** -60, t, scale=0.5, top=3)
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
+    f[3, 0] = INF                                                      # counts: the row is NaN, no other
+    r = nemo_amd.bank_log_probs(f, b, t, scale=0.5, top=3)
+    assert bool(torch.isnan(r.lse[3])) and int(r.top_index[3, 0]) == -1
+    keep = torch.arange(100, device=gpu) != 3
+    assert all(torch.equal(x[keep], y[keep]) for x, y in zip(p, r))
 
 
 @pytest.mark.gpu
@@ -750,6 +828,37 @@ def test_other_stream_and_captured_graph(gpu):
         assert all(torch.equal(p, q) for p, q in zip(got, step())), f"replay {i}"
 
 
+@pytest.mark.gpu
+def test_two_graphs_and_calls_without_gradients(gpu):
+    """Two captured graphs replayed in turn, each with its own workspace; results without gradients are those with them."""
+    import nemo_amd
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    data = [(torch.randn(S, 48, generator=gen, device=gpu).requires_grad_(), torch.randn(V, 48, generator=gen, device=gpu).requires_grad_(),
+             torch.randint(0, V, (S,), generator=gen, device=gpu)) for S, V in ((70, 301), (500, 90))]
+
+    def step(x, bank, t):
+        y = nemo_amd.linear(x, bank, alpha=0.1)
+        r, q = nemo_amd.bank_log_probs(x, bank, t, scale=0.1, top=2), nemo_amd.log_probs(y, t, top=2)
+        return [*r, *q, *torch.autograd.grad((r.logp + q.entropy).sum(), (x, bank))]
+    eager = [[o.detach().clone() for o in step(*d)] for d in data]
+    with torch.no_grad():
+        for (x, bank, t), e in zip(data, eager):
+            free = [*nemo_amd.bank_log_probs(x, bank, t, scale=0.1, top=2), *nemo_amd.log_probs(nemo_amd.linear(x, bank, alpha=0.1), t, top=2)]
+            assert not any(o.requires_grad for o in free) and all(torch.equal(p, q) for p, q in zip(free, e))
+    graphs = []
+    for d in data:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*d)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), e in zip(graphs, eager):
+            assert all(torch.equal(p.detach(), q) for p, q in zip(out, e))
+
+
 # ---- the C entries' refusals (no launch happens: run on the CPU) ----------------------------------------------------------
 def _lib_or_skip():
     import os
@@ -795,9 +904,22 @@ def test_entry_refusals():
     assert lib.nemo_linear_workspace(p, 8, p, 8, 4, 4, 8, 0) == 0       # aligned rows and enough tiles' worth of nothing to split
 
 
+def test_entry_refuses_strides():
+    lib = _lib_or_skip()
+    p = C.c_void_p(4096)
+    assert lib.nemo_linear(p, 1 << 21, p, 8, None, None, 0, 4, 4, 8, 0, 0, 1.0, 1.0, p, None, None, 0, None) == -2
+    assert "4 MiB" in lib.nemo_last_error().decode()
+    assert lib.nemo_bank_log_probs_backward(p, 16, p, 16, p, 1 << 28, p, p, None, None, None, 4, 9, 16, 0, 1.0, 0, p, p, p, 1 << 30, None) == -2
+    assert "2^27" in lib.nemo_last_error().decode()
+
+
 def test_host_tensors_are_refused():
     import nemo_amd
     x, t = torch.zeros(4, 16), torch.zeros(4, dtype=torch.int64)
     for call in (lambda: nemo_amd.linear(x, x), lambda: nemo_amd.log_probs(x, t), lambda: nemo_amd.bank_log_probs(x, x, t)):
         with pytest.raises(RuntimeError, match="CPU"):
+            call()
+    for call in (lambda: nemo_amd.linear(None, x), lambda: nemo_amd.linear([1.0], x), lambda: nemo_amd.log_probs(None, t),
+                 lambda: nemo_amd.bank_log_probs(None, x, t)):
+        with pytest.raises(TypeError):
             call()
