@@ -92,6 +92,18 @@ template <int NP, int CP> struct Stager {
                 copy_to_lds(in ? (const void*)(p + n * CP) : (const void*)&g_zero_row, lds + n * L::BYTES + (i * 4 + wave) * L::PITCH);
         }
     }
+    // A tile of the first n of the rows in `list`, zeros behind them.
+    __device__ inline void gather(char* lds, const BankArgs& a, const int* list, int n, int lane) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (i * 4 + wave) * L::RPI + lane / L::CPR, c = (lane & (L::CPR - 1)) ^ L::flip(r);
+            const bool in = r < n && c * 8 < a.channels;
+            const bf16* p = a.other + (in ? (long)list[r] : 0) * a.ld_other + c * 8;
+#pragma unroll
+            for (int k = 0; k < NP; ++k)
+                copy_to_lds(in ? (const void*)(p + k * CP) : (const void*)&g_zero_row, lds + k * L::BYTES + (i * 4 + wave) * L::PITCH);
+        }
+    }
 };
 
 // Fragment kf of the tile's rows, one piece.
