@@ -4,6 +4,8 @@ rows with entropy and best alternatives (`log_probs`), and both joined without t
 The reference computes this loss in torch from FeatureBankNeMo's similarity and MaskCreater's weights (nemo/models/nemo.py:138-209):
 softmax over the bank's rows of similarity / T - weight, cross entropy at the slot's own row.  All functions are differentiable (once),
 run on the current stream of their tensors' device, never synchronise, and raise before any launch on arguments they do not take.
+They may be captured into a graph, with their backward pass too; as with torch's own operators no eager autograd graph of the same leaves may
+be alive then (the leaves' gradients would be gathered on the stream of that graph, outside the capture): drop its results first.
 """
 from collections import namedtuple
 

@@ -15,8 +15,14 @@
 // fragments are read with the transposing LDS read, 32 bytes of a row at a time, and those 32-byte pieces are spread over the banks by
 // an exclusive-or with the k row.
 //
-// Operands must start on 16 bytes, have rows that start on 16 bytes and a contiguous extent of whole 16 bytes; others are first copied
-// into the workspace with padded rows (pack_kernel).
+// The copies to LDS need operands that start on 16 bytes, with rows that do and a contiguous extent of whole 16 bytes; others are first copied into
+// the workspace with padded rows (pack_kernel).  Bias, residual and results may start at any element.
+//
+// Measured (a call).  8192 x 4096 x 4096 bf16 with gelu, bias and residual: 255 us, 1078 TF; the bare product of a library 207 us, 1326 TF.
+// 160000 x 128 x 2048 bf16 with relu and bias (696 MB): 177 us, 3.9 TB/s.  5590 x 15976 x 128 f32 with a residual: 268 us, 86 TF and 2.7 TB/s:
+// the f32 matrix instructions alone take 149 us, reading and writing the 714 MB alone 150, and little of the two overlaps.
+// 8191 x 1001 x 515 f16, rows off 16 bytes, silu, bias, residual: packing 6, product 33 us; backward: packing 6, slope 20, column sums 5,
+// products 24 and 22 + 6 (join).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -426,8 +432,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob first, PackJob second
 }
 
 // dz = dy act'(pre) (rounded to T because the matrix cores take T), dr = beta dy, and per block of rows the column sums of the unrounded
-// dz (for the bias).  A workgroup takes 256 columns x ROWS rows: 32 threads of eight columns, eight rows at a time.  Bound by memory; rows
-// may start at any element.
+// dz (for the bias).  A workgroup takes 256 columns x kSlopeRows rows: 32 threads of eight columns, eight rows at a time.  Bound by the latency of
+// its loads: 8191 x 1001 f16 (49 MB) 20 us with 32 rows a workgroup, 25 with 64; 18 where rows start on 16 bytes.
 constexpr int kSlopeRows = 32;
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const T* dy, long ldg, const T* pre, long ldpre, long m, int n, int act, float beta,

@@ -602,6 +602,17 @@ def test_bank_log_probs_scores_far_below_zero(gpu, scale, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["none", "rows"])
+@pytest.mark.parametrize("S,V,ch", [(45000, 3, 16), (3000, 300, 40), (1500, 140, 256)])
+def test_bank_log_probs_many_rows_of_few_targets(gpu, S, V, ch, kind, dtype):
+    """More rows of one target than one look of a workgroup finds, numbers that are no multiple of a tile, and rows without a target."""
+    gen = torch.Generator(device=gpu).manual_seed(S)
+    t = torch.randint(-1, 3, (S,), generator=gen, device=gpu)
+    bank_case(gpu, S, V, ch, TYPES[dtype], kind, 0, targets=t)
+
+
+@pytest.mark.gpu
 def test_bank_log_probs_far_apart_magnitudes_and_repeated_targets(gpu):
     """f32 rows as pieces: powers of two of the rows change no bit.  All slots share two targets."""
     import nemo_amd
