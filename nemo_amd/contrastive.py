@@ -34,7 +34,20 @@ def _device_tensors(what, dtypes, names, *tensors):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _once(gradients):
+    """`gradients` as a backward pass that is not differentiable itself; what that takes is only paid where a graph of it is asked for."""
+    guarded = once_differentiable(gradients)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else gradients(ctx, *grads)
+    return backward
 
 
 def _number(what, name, value):
@@ -55,7 +68,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y):
         x, weight, pre = ctx.saved_tensors
         activation, alpha, beta = ctx.args
@@ -149,7 +162,7 @@ class _LogProbs(torch.autograd.Function):
         return _results(out)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g_logp, g_entropy, g_lse, *_):
         logits, targets, weights, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:
@@ -191,7 +204,7 @@ class _BankLogProbs(torch.autograd.Function):
         return _results(out)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g_logp, g_entropy, g_lse, *_):
         features, bank, targets, weights, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:

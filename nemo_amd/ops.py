@@ -5,6 +5,7 @@ current stream, and raises on a non-zero return code.  No arithmetic happens her
 """
 import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -724,6 +725,12 @@ def _raw(t):
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(entry, *sizes):
+    """Bytes that `entry`_workspace asks for: a function of sizes, strides and of the pointers' last four bits (given in their place)."""
+    return getattr(_lib.load(), entry + "_workspace")(*sizes)
+
+
 def _scratch(nbytes, device):
     """Workspace of a call; freed after it, which on one stream is in order."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
@@ -745,7 +752,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     pre = torch.empty((M, N), dtype=x.dtype, device=dev) if want_pre else None
     px, pw = x.data_ptr(), weight.data_ptr()
     with _on(dev):
-        nbytes = lib.nemo_linear_workspace(px, ldx, pw, ldw, M, N, K, dt)
+        nbytes = _workspace("nemo_linear", px & 15, ldx, pw & 15, ldw, M, N, K, dt)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_linear(px, ldx, pw, ldw, _raw(bias), _raw(residual), ldr, M, N, K, dt, ACTIVATIONS[activation], alpha, beta, y.data_ptr(),
                               _raw(pre), _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_linear")
@@ -766,7 +773,7 @@ def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1
     outs = [empty(s, dtype=grad_y.dtype, device=dev) if w else None for s, w in zip(shapes, want)]
     pg, px, pw, act = grad_y.data_ptr(), _raw(x), _raw(weight), ACTIVATIONS[activation]
     with _on(dev):
-        nbytes = lib.nemo_linear_backward_workspace(pg, ldg, px, ldx, pw, ldw, M, N, K, dt, act)
+        nbytes = _workspace("nemo_linear_backward", pg & 15, ldg, px and px & 15, ldx, pw and pw & 15, ldw, M, N, K, dt, act)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_linear_backward(pg, ldg, px, ldx, pw, ldw, _raw(pre), M, N, K, dt, act, alpha, beta, *[_raw(o) for o in outs], _raw(ws),
                                        nbytes, _raw_stream(dev.index)), "nemo_linear_backward")
@@ -811,7 +818,7 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0, want_stats=True):
     dev = logits.device
     out = _Probs(S, top, want_stats, dev)
     with _on(dev):
-        nbytes = lib.nemo_log_probs_workspace(S, V, top)
+        nbytes = _workspace("nemo_log_probs", S, V, top)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_log_probs(logits.data_ptr(), ld, _raw(weights), ldw, targets.data_ptr(), S, V, DTYPES[logits.dtype], scale, top,
                                  *out.pointers(), _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_log_probs")
@@ -847,7 +854,7 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0, want
     out = _Probs(S, top, want_stats, dev)
     pf, pb = features.data_ptr(), bank.data_ptr()
     with _on(dev):
-        nbytes = lib.nemo_bank_log_probs_workspace(pf, ldf, pb, ldb, S, V, ch, dt, top)
+        nbytes = _workspace("nemo_bank_log_probs", pf & 15, ldf, pb & 15, ldb, S, V, ch, dt, top)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_bank_log_probs(pf, ldf, pb, ldb, _raw(weights), ldw, targets.data_ptr(), S, V, ch, dt, scale, top, *out.pointers(),
                                       _raw(ws), nbytes, _raw_stream(dev.index)), "nemo_bank_log_probs")
@@ -868,7 +875,7 @@ def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_e
     grads = [empty((n, ch), dtype=features.dtype, device=dev) if w else None for n, w in zip((S, V), want)]
     pf, pb = features.data_ptr(), bank.data_ptr()
     with _on(dev):
-        nbytes = lib.nemo_bank_log_probs_backward_workspace(pf, ldf, pb, ldb, S, V, ch, dt)
+        nbytes = _workspace("nemo_bank_log_probs_backward", pf & 15, ldf, pb & 15, ldb, S, V, ch, dt)
         ws = _scratch(nbytes, dev)
         check(lib.nemo_bank_log_probs_backward(pf, ldf, pb, ldb, _raw(weights), ldw, targets.data_ptr(), stats.data_ptr(),
                                                *[_raw(g) for g in gs], S, V, ch, dt, scale, top, *[_raw(g) for g in grads], _raw(ws), nbytes,
