@@ -12,6 +12,7 @@
 // best: 7.5 us, the latency of a launch, of a few dependent loads and of five selections.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/nemo_hip.h"
@@ -296,11 +297,12 @@ __global__ __launch_bounds__(256) void log_probs_backward_kernel(LogProbArgs a, 
 
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Parts of a row where there are too few rows to fill the device: four workgroups a compute unit, at least 8192 columns a part.
+// Parts of a row where there are too few rows to fill the device: four workgroups a compute unit, at least 8192 columns a part, rows of at least
+// four of them (the join is a launch).  Measured in us, f32, parts of 2048 / 8192 / 32768 columns: 16 x 20000 6.3 / 6.7 / 5.9 (one part),
+// 128 x 16384 6.8 / 6.6 / 5.0 (one part), 16 x 130000 7.0 / 6.7 / 10.1, 1 x 130000 with the five best 11.9 / 12.5 / 16.1.
 static int parts_of(int64_t rows, int64_t cols) {
-    int64_t p = rows > 0 ? 1024 / rows : 1;
-    if (p > cols / 8192) p = cols / 8192;
-    return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
+    if (rows <= 0 || cols < 4 * 8192) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(64, std::min(1024 / rows, cols / 8192)));
 }
 
 static int check_log_probs(const char* who, int64_t rows, int64_t cols, int dtype, int top) {
@@ -313,8 +315,10 @@ static int check_log_probs(const char* who, int64_t rows, int64_t cols, int dtyp
 
 template <typename T>
 static void launch_log_probs(const LogProbArgs& a, hipStream_t st) {
-    // One wave a row where a row is short and there are enough of them to fill the device that way; four waves a row otherwise.
-    const bool narrow = a.cols <= 2048 && a.rows >= 2048;
+    // One wave a row where there is a row for every SIMD and it is no longer than 32 KB; else four waves a row.  Measured in us, four waves / one:
+    // f32 2048 x 500 5.4 / 4.0, 8000 x 1118 with the five best 43.7 / 20.4, 32768 x 4000 with them 192 / 123, 8000 x 8000 with them 64 / 60, 8000 x 13416
+    // with them 93 / 95, 16000 x 16384 183 / 194, 1024 x 8000 8.2 / 9.0; bf16 8000 x 13416 with the five best 80 / 56, 4096 x 60000 95 / 97.
+    const bool narrow = a.rows >= 1024 && (int64_t)a.cols * (int64_t)sizeof(T) <= 32768;
     const unsigned wgs = narrow ? (unsigned)((a.rows + 3) / 4) : (unsigned)(a.rows * a.parts);
     auto launch = [&](auto top, auto weighted) {
         constexpr bool TOP = decltype(top)::value, W = decltype(weighted)::value;

@@ -784,6 +784,8 @@ def _row_weights(weights, cols):
     """(tensor, row stride) of log-prob weights: None, one row for all ([cols], stride 0) or a row each."""
     if weights is None:
         return None, 0
+    if weights.dim() == 2 and weights.shape[0] > 1 and weights.stride(0) == 0:
+        weights = weights[0]                                                # one row expanded
     if weights.dim() == 1:
         return weights.contiguous(), 0
     return rows_2d(weights, cols)

@@ -366,7 +366,7 @@ def log_probs_case(dev, S, V, dtype, kind, top, scale=0.5, which="logp entropy l
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("kind", ["none", "bank", "rows"])
-@pytest.mark.parametrize("S,V", [(1, 1), (1, 7), (2, 64), (5, 1118), (3, 1031), (70, 2049), (1, 40003), (3, 70001), (2500, 33)])
+@pytest.mark.parametrize("S,V", [(1, 1), (1, 7), (2, 64), (5, 1118), (3, 1031), (70, 2049), (1, 40003), (3, 70001), (2500, 33), (1100, 1500)])
 def test_log_probs_sizes(gpu, S, V, kind, dtype):
     log_probs_case(gpu, S, V, TYPES[dtype], kind, 0 if V % 2 else 5)
     log_probs_case(gpu, S, V, TYPES[dtype], kind, 16 if V % 2 else 1, seed=1)
