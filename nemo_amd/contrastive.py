@@ -92,7 +92,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     x [..., K], weight [N, K], bias [N], residual [..., N] of one type (float32, bfloat16 or float16) -> [..., N] of that type.
     activation: "none", "relu", "gelu" (the exact one, with erf) or "silu".  Products are summed in 32 bits (float32: on the f32 matrix
     cores, so infinities and NaN come out as in any f32 product) and the result is rounded once.  x, weight, bias and residual are
-    differentiable.  Rows of x, weight and residual may be strided; alignment matters for speed only."""
+    differentiable.  Rows of x, weight and residual may be strided; alignment matters for speed only.  Rows of x and weight take up to 4 MiB."""
     _device_tensors("linear", ops.DTYPES, ("x", "weight", "bias", "residual"), x, weight, bias, residual)
     if activation not in ops.ACTIVATIONS:
         raise ValueError(f"linear: activation {activation!r} (takes {', '.join(ops.ACTIVATIONS)})")

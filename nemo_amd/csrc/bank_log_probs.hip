@@ -170,7 +170,7 @@ using namespace nemo;
 
 extern "C" size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,
                                                 int64_t channels, int32_t dtype, int32_t top) {
-    if (rows <= 0 || cols < 0 || channels <= 0 || channels > 256) return 0;
+    if (rows <= 0 || cols < 0 || channels <= 0 || channels > 256 || top < 0 || top > kMaxTop) return 0;
     const Parts p = forward_parts(rows, cols, padded_channels((int)channels), dtype);
     return rows_bytes(features, ldf, rows, channels, dtype) + rows_bytes(bank, ldb, cols, channels, dtype) +
            align256((size_t)3 * 2 * p.parts * rows * 4) + 2 * align256((size_t)2 * p.parts * rows * top * 4) + align256((size_t)rows * 4);

@@ -338,7 +338,7 @@ using namespace nemo;
 
 extern "C" size_t nemo_log_probs_workspace(int64_t rows, int64_t cols, int32_t top) {
     const int parts = parts_of(rows, cols);
-    if (rows <= 0 || parts <= 1) return 0;
+    if (rows <= 0 || parts <= 1 || top < 0 || top > kMaxTop) return 0;
     return align256((size_t)3 * parts * rows * 4) + align256((size_t)parts * rows * top * 4) * 2;
 }
 
