@@ -431,7 +431,7 @@ int nemo_mask_weight(const int32_t* object_idx, const int32_t* source_vert_idx, 
 /* y[M,N] = act(alpha x[M,K] weight[N,K]^T + bias[N]) + beta residual[M,N].  All tensors of one element type; products are
  * summed in f32 and the result is rounded once.  activation: 0 none, 1 relu, 2 gelu (with erf), 3 silu.  bias, residual
  * may be NULL.  pre [M,N] or NULL: alpha x W^T + bias in the element type, what nemo_linear_backward needs when there is an
- * activation.  K = 0 gives act(bias) + beta residual.  workspace: nemo_linear_workspace bytes of device memory
+ * activation (for all but grad_residual).  K = 0 gives act(bias) + beta residual.  workspace: nemo_linear_workspace bytes of device memory
  * (asked with the same pointers and strides: operands whose rows are not aligned to 16 bytes are copied into it), contents
  * undefined before and after.  Rows of the two operands (and of grad_y below) may lie up to 4 MiB apart, a matrix may have 2^34 elements. */
 size_t nemo_linear_workspace(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K, int32_t dtype);

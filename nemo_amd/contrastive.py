@@ -51,6 +51,8 @@ def _once(gradients):
 
 
 def _number(what, name, value):
+    if torch.is_tensor(value):
+        raise TypeError(f"{what}: {name} must be a number, not a tensor (it is read on the host and has no gradient)")
     value = float(value)
     if value != value or value in (float("inf"), -float("inf")):
         raise ValueError(f"{what}: {name} must be finite, got {value}")

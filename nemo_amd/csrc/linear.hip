@@ -748,6 +748,7 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
     if (rc) return rc;
     if (M > 0 && N > 0 && !grad_y) return fail(NEMO_ERR_INVALID, "nemo_linear_backward: null gradient");
     if (M > 0 && N > 0 && ldg < N) return fail(NEMO_ERR_INVALID, "nemo_linear_backward: a row stride shorter than the row");
+    if (!grad_x && !grad_weight && !grad_bias) activation = ACT_NONE;        // the residual's gradient passes the activation by
     if (activation != ACT_NONE && M > 0 && N > 0 && !pre) return fail(NEMO_ERR_INVALID, "nemo_linear_backward: the activation needs `pre`");
     if (M > 0 && N > 0 && K > 0 && ((grad_x && (!weight || ldw < K)) || (grad_weight && (!x || ldx < K))))
         return fail(NEMO_ERR_INVALID, "nemo_linear_backward: null operand or a row stride shorter than the row");

@@ -697,7 +697,7 @@ def spherical_angles(campos):
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _SAME_DEVICE = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # absent from a torch without GPU support, which has nothing to launch
 
 
 def _on(device):

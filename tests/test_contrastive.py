@@ -359,7 +359,7 @@ def log_probs_case(dev, S, V, dtype, kind, top, scale=0.5, which="logp entropy l
     (gx,) = run_grads(r, g, [logits])
     assert gx.dtype == dtype and gx.shape == (S, V)
     want = scale * ref["dz"][:, :V]
-    b = scale * bounds["dz"][:, :V]
+    b = abs(scale) * bounds["dz"][:, :V]
     within(gx, want, b + half_step(dtype) * (want.abs() + b) + tiny(dtype) * 2 * (want != 0), "gradient of logits")
 
 
@@ -376,6 +376,36 @@ def test_log_probs_sizes(gpu, S, V, kind, dtype):
 @pytest.mark.parametrize("which", ["logp", "entropy", "lse", "logp lse"])
 def test_log_probs_single_gradients(gpu, which):
     log_probs_case(gpu, 40, 301, torch.float32, "rows", 0, which=which)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-2.0, 0.0, 1e-35, 50.0])
+@pytest.mark.parametrize("kind", ["none", "rows"])
+def test_log_probs_scales(gpu, kind, scale):
+    log_probs_case(gpu, 30, 1500, torch.float32, kind, 0 if scale == 1e-35 else 5, scale=scale)
+    log_probs_case(gpu, 1100, 700, torch.bfloat16, kind, 0, scale=scale)
+
+
+@pytest.mark.gpu
+def test_gradients_of_some_inputs_only(gpu):
+    """One input at a time needs a gradient; gradients come from sums (expanded, stride 0); weights are one row expanded."""
+    import nemo_amd
+    gen = torch.Generator(device=gpu).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=gpu)
+    args = {"x": rnd(60, 70), "weight": rnd(90, 70), "bias": rnd(90), "residual": rnd(60, 90)}
+    full = {k: v.clone().requires_grad_() for k, v in args.items()}
+    want = dict(zip(full, torch.autograd.grad(nemo_amd.linear(**full, activation="silu", beta=0.5).sum(), list(full.values()))))
+    for k in args:
+        leaf = args[k].clone().requires_grad_()
+        (got,) = torch.autograd.grad(nemo_amd.linear(**{**args, k: leaf}, activation="silu", beta=0.5).sum(), leaf)
+        assert torch.equal(got, want[k]), k
+    f, b, t, w = rnd(60, 32), rnd(90, 32), torch.randint(0, 90, (60,), generator=gen, device=gpu), torch.rand(1, 90, generator=gen, device=gpu)
+    F, B = f.clone().requires_grad_(), b.clone().requires_grad_()
+    r = nemo_amd.bank_log_probs(F, B, t, w.expand(60, 90), scale=0.3)
+    wf, wb = torch.autograd.grad(r.logp.sum(), (F, B), retain_graph=True)
+    assert torch.equal(torch.autograd.grad(nemo_amd.bank_log_probs(F, b, t, w[0], scale=0.3).logp.sum(), F)[0], wf)
+    assert torch.equal(torch.autograd.grad(nemo_amd.bank_log_probs(f, B, t, w.expand(60, 90).contiguous(), scale=0.3).logp.sum(), B)[0], wb)
+    assert torch.equal(torch.autograd.grad(r.logp.sum(), B)[0], wb)
 
 
 def special_rows(dev):
@@ -511,7 +541,7 @@ def test_log_probs_refusals(gpu):
                     dict(top=1.5), dict(scale=INF), dict(weights=torch.zeros(9, device=gpu, requires_grad=True))):
             with pytest.raises(ValueError):
                 call(**bad)
-        for bad in (dict(t=t.float()), dict(weights=torch.zeros(9, device=gpu).half())):
+        for bad in (dict(t=t.float()), dict(weights=torch.zeros(9, device=gpu).half()), dict(scale=torch.ones((), device=gpu))):
             with pytest.raises(TypeError):
                 call(**bad)
         with pytest.raises(RuntimeError):
