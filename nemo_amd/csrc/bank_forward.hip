@@ -109,11 +109,11 @@ __global__ __launch_bounds__(256, NP * CP > 512 ? 1 : 2) void bank_forward_kerne
     // tiles from `t` on one step after the other, with every precaution
     auto plain_pass = [&](int t) __attribute__((always_inline)) {
         for (; t < t1; ++t) {
-            __syncthreads();
+            publish_lds();
             stage(lds0, t);
             float wv[16], v[16];
             load_weights(wv, t);
-            __syncthreads();
+            publish_lds();
             const f32x16_t pr = products<NP, CP>(lds0, q, lane);
             const int left = a.n_other - t * 32 - 4 * g;               // registers whose row 8 b + i is at least this are beyond the end
 #pragma unroll
@@ -130,14 +130,14 @@ __global__ __launch_bounds__(256, NP * CP > 512 ? 1 : 2) void bank_forward_kerne
     const int whole = t1 == tiles && a.n_other % 32 != 0 && t1 > t0 ? t1 - 1 : t1;
     if (t0 < whole) {
         stage(lds0, t0);
-        __syncthreads();
+        publish_lds();
         f32x16_t pr = products<NP, CP>(lds0, q, lane);
         stage(lds1, t0 + 1);
         // `next` holds tile t + 1; `after` held tile t, whose products are in pr.  A slice: a fragment is read (two slices ahead of its use),
         // multiplied, and a share of the 18 units of tile t is done: the largest product, the state raised to it, 16 products added.  Weights
         // may arrive during the first half of the slices.
         auto step = [&](int t, const char* next, char* after) __attribute__((always_inline)) {
-            __syncthreads();                                           // tile t + 1 is there; nobody reads tile t any more
+            publish_lds();                                             // tile t + 1 is there; nobody reads tile t any more
             stage(after, t + 2);                                       // also behind the part's last tile, to no effect: no branch
             float wv[16], v[16];
             load_weights(wv, t);
@@ -190,6 +190,7 @@ __global__ __launch_bounds__(256, NP * CP > 512 ? 1 : 2) void bank_forward_kerne
             step(t + 1, lds0, lds1);
         }
         if (t < whole) step(t, lds1, lds0);
+        wait_for_copies();                                             // of the tiles behind the last one: no wave ends before they are there
     }
     plain_pass(whole);
     if (!GENERAL) {

@@ -224,11 +224,11 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
         };
         if (t0 < t1) stage(lds0, s_coef0, t0);
         for (int t = t0; t < t1; t += 2) {
-            __syncthreads();
+            publish_lds();
             if (t + 1 < t1) stage(lds1, s_coef1, t + 1);
             one(lds0, s_coef0, t);
             if (t + 1 >= t1) break;
-            __syncthreads();
+            publish_lds();
             if (t + 2 < t1) stage(lds0, s_coef0, t + 2);
             one(lds1, s_coef1, t + 1);
         }
@@ -242,11 +242,11 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
         for (int i = threadIdx.x * 16; i < NP * L::BYTES; i += 4096) *(u32x4*)(lds3 + i) = u32x4{0, 0, 0, 0};
         stage(lds0, s_coef0, t0);
         if (t0 + 1 < t1) stage(lds1, s_coef1, t0 + 1);
-        __syncthreads();
+        publish_lds();
         f32x16_t pr = products<NP, CP>(lds0, q, lane);
         auto step = [&](int t, const char* before, const char* next, char* after, const float (*coef)[64],
                         float (*coef_after)[64]) __attribute__((always_inline)) {
-            __syncthreads();                                           // tile t + 1 is there; nobody reads tile t - 2 any more
+            publish_lds();                                             // tile t + 1 is there; nobody reads tile t - 2 any more
             stage(after, coef_after, t + 2);                           // also behind the part's last tile, to no effect: no branch
             float wv[16];
             load_weights(wv, t);
@@ -317,14 +317,14 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
         constexpr int SCAN = 4;                                        // rows a thread looks at in one go
         int listed = 0;
         auto multiply = [&](int n) __attribute__((always_inline)) {    // the first n (at most 32) of the list
-            __syncthreads();
+            publish_lds();
             if (threadIdx.x < 32) {
                 const int r = (int)threadIdx.x < n ? s_list[threadIdx.x] : 0;
                 s_target[threadIdx.x] = (int)threadIdx.x < n ? __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + r]) : -1;
                 s_share[threadIdx.x] = a.coef[K_LOGP * n_coef + r];
             }
             stager.gather(lds0, a, s_list, n, lane);
-            __syncthreads();
+            publish_lds();
             const int t = s_target[lane & 31];
             if (__any(t >= own0 && t < own0 + 32)) {
                 float z[16];
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
                 const int t = r < end ? __builtin_bit_cast(int, a.coef[K_TARGET * n_coef + r]) : -1;
                 found[i] = __ballot(t >= first_owner && t < first_owner + 128);
             }
-            __syncthreads();                                           // nobody reads the list or the counts any more
+            publish_lds();                                             // nobody reads the list or the counts any more
             if (lane == 0)
 #pragma unroll
                 for (int i = 0; i < SCAN; ++i) s_found[i * 4 + wave] = __builtin_popcountll(found[i]);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
 #pragma unroll 1
             while (listed >= 32 || (last && listed > 0)) {
                 multiply(min(listed, 32));
-                __syncthreads();
+                publish_lds();
                 int keep[SCAN];                                        // the rest moves to the front
 #pragma unroll
                 for (int i = 0; i < SCAN; ++i) keep[i] = s_list[32 + i * 256 + threadIdx.x];
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
 #pragma unroll
         for (int i = 0; i < 16; ++i) broken |= !(__builtin_fabsf(acc[x][i]) <= FLT_MAX);
     if (threadIdx.x == 0) s_again = 0;
-    __syncthreads();                                                   // also: nobody reads the tiles any more
+    publish_lds();                                                     // also: nobody reads the tiles any more, and no copy is under way
     if (broken) s_again = 1;
     __syncthreads();
     if (s_again) {

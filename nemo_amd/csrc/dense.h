@@ -78,6 +78,17 @@ __device__ inline void copy_words_to_lds(const void* g, void* lds) {
     __builtin_amdgcn_global_load_lds((NEMO_GLOBAL void*)g, (NEMO_LDS void*)lds, 4, 0, 0);
 }
 
+// The copies are asynchronous: a wave waits here for its own.
+__device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A barrier behind which other waves read what this one has copied or written to LDS, or copy over what it has read.  __syncthreads alone does not wait
+// for copies, and around a loop not always for writes either: the compiler leaves the wait out in front of a barrier whose copies it has not
+// seen yet when it gets there, those of the loop's last turn.
+__device__ inline void publish_lds() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // ---- reductions -----------------------------------------------------------------------------------------------------------------
 // Over the 64 lanes of a wave, all of them active, with the lane permutations of the vector units (a tenth of the latency of exchanges through
 // LDS): within four, eight and sixteen lanes, then lane 15 of a row of sixteen into the next one, lane 31 into the upper half; lane 63 has it all.

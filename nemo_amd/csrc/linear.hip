@@ -291,13 +291,13 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 1 : BQ == 128 ? 2 : BQ ==
         };
         auto step = [&](char* here, const char* next, int t, auto any_tag) __attribute__((always_inline)) {
             multiply(0, here, 1);
-            __syncthreads();                                           // the next tile is there, nobody reads this one any more
+            publish_lds();                                             // the next tile is there, nobody reads this one any more
             if constexpr (decltype(any_tag)::value) load_any(here, t + 2);
             else load(here, t + 2);
             multiply(1, next, 0);                                      // behind the last tile what is read is of no use, and none is made of it
         };
         load_any(lds0, 0);
-        __syncthreads();
+        publish_lds();
         load_any(lds1, 1);
 #pragma unroll
         for (int n = 0; n < HALF * (NP + NQ); ++n) read(lds0, 0, n);
