@@ -194,8 +194,8 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
         constexpr bool SAFE = decltype(safe_tag)::value || GENERAL;
         const float s = !GENERAL ? pr[i] : w ? score(pr[i], a.scale, wv[i]) : score(pr[i], a.scale);
         const float d = pair_gradient<F32, GENERAL, SAFE>(s, k, k4.m[i & 3], k4.s[i & 3], k4.c[i & 3], k4.g2[i & 3]);
-        // rows beyond the last are zeros, but where all scores are far below 0 the probability of a 0 is not even finite
-        return SAFE && !GENERAL && !OWN_BANK && tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= a.n_other ? 0.0f : d;
+        // rows beyond the last are zeros (with weights, left out), but where all scores are far below 0 the probability of a 0 is not even finite
+        return decltype(safe_tag)::value && !OWN_BANK && !(GENERAL && w) && tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= a.n_other ? 0.0f : d;
     };
     const int tiles = (a.n_other + 31) / 32;
     const int t0 = part * a.part_tiles, t1 = min(tiles, t0 + a.part_tiles);
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256, CP == 256 || (CP == 128 && sizeof(T) == 4) ? 1
 #pragma unroll
     for (int x = 0; x < NX; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) broken |= !(__builtin_fabsf(acc[x][i]) <= FLT_MAX);
+        for (int i = 0; i < 16; ++i) broken |= live && !(__builtin_fabsf(acc[x][i]) <= FLT_MAX);
     if (threadIdx.x == 0) s_again = 0;
     publish_lds();                                                     // also: nobody reads the tiles any more, and no copy is under way
     if (broken) s_again = 1;
