@@ -97,12 +97,16 @@ struct GemmArgs {
     Epilogue e;
 };
 
-// Rounds to T; for the stored pre-activation of f16 a value that rounds to zero keeps its sign as the smallest subnormal, so that relu's
-// slope is that of the value before rounding.
-template <typename T> __device__ inline T round_pre(float z) { return (T)z; }
-template <> __device__ inline f16 round_pre<f16>(float z) {
-    const f16 h = (f16)z;
-    if (h == (f16)0.0f && z != 0.0f) return z > 0.0f ? (f16)5.9604644775390625e-8f : (f16)-5.9604644775390625e-8f;
+// The stored pre-activation: rounds to T so that the slopes stay those of the value before rounding.  A finite value beyond T's largest is kept as
+// that one (an infinity would make the slopes of gelu and silu 0 x infinity; out there they are 0 and 1), and one that f16 rounds to zero keeps
+// its sign as the smallest subnormal (relu).
+template <typename T> __device__ inline T round_pre(float z) {
+    if constexpr (sizeof(T) == 4) return z;
+    constexpr bool F16 = std::is_same<T, f16>::value;
+    constexpr float most = F16 ? 65504.0f : 3.3895313892515355e38f;
+    const float cut = __builtin_amdgcn_fmed3f(z, -most, most);
+    const T h = (T)(__builtin_fabsf(z) <= __FLT_MAX__ ? cut : z);
+    if (F16 && h == (T)0.0f && z != 0.0f) return z > 0.0f ? (T)5.9604644775390625e-8f : (T)-5.9604644775390625e-8f;
     return h;
 }
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_contrastive import TYPES, bank_case
+from tests.test_contrastive import ACT, CURVE, INF, TYPES, U, bank_case, half_step, tiny, within
 
 
 @pytest.mark.gpu
@@ -19,3 +19,55 @@ def test_scores_far_below_zero_with_a_list(gpu, S, V, ch, scale, dtype):
     for top in (1, 5, 16):
         bank_case(gpu, S, V, ch, TYPES[dtype], "none", top, scale=scale, features=f, bank=b)
     bank_case(gpu, S, V, ch, TYPES[dtype], "rows", 5, scale=scale, features=f, bank=b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_linear_pre_activations_beyond_f16(gpu, act):
+    """Half of the pre-activations lie beyond the largest f16, where the slopes are 0 and 1 (to far more than 64 bits); the results on the negative side
+    are the residual, and every gradient is what 64 bits give.  The others are ordinary: their slopes are off by the rounding of the kept
+    pre-activation (half a step) times the curvature."""
+    import nemo_amd
+    M, N, K, dt = 50, 36, 8, torch.float16
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=gpu)
+    x, w = rnd(M, K), rnd(N, K) * K ** -0.5
+    x[:, 0], w[:, 0] = 0, 0
+    x[:, 0] = torch.where(torch.arange(M, device=gpu) % 2 == 0, 300.0, -240.0)
+    w[::2, 0] = 280.0                                                  # 84000 and -67200
+    x, w, r, g = (t.to(dt) for t in (x, w, rnd(M, N), rnd(M, N)))
+    leaves = [t.clone().requires_grad_() for t in (x, w, torch.zeros(N, device=gpu, dtype=dt), r)]
+    y = nemo_amd.linear(*leaves, activation=act)
+    grads = torch.autograd.grad(y, leaves, g)
+    X, W, G, uT = x.double(), w.double(), g.double(), half_step(dt)
+    z = (X @ W.T).requires_grad_()
+    (slope,) = torch.autograd.grad(ACT[act](z).sum(), z)
+    z = z.detach()
+    far = z.abs() > 1000
+    assert bool((z.abs()[far] > 65520).all()) and int(far.sum()) == M * N // 2 and bool((far & (z < 0)).any())
+    assert torch.equal(y.detach()[far & (z < 0)], r[far & (z < 0)]) and bool((y[far & (z > 0)] == INF).all())
+    z_err = (K + 4) * U * (X.abs() @ W.abs().T)
+    s_err = CURVE[act] * (z_err + uT * z.abs() + tiny(dt)) + 16 * U * (1 + z.abs())
+    if act == "relu":
+        s_err = (z.abs() <= z_err).double()
+    s_err = torch.where(far, torch.zeros_like(z), s_err)
+    dz, e = G * slope, G.abs() * s_err
+    dz_err = e + uT * (dz.abs() + e) + tiny(dt)                        # dz is rounded in front of the two products
+    want = (dz @ W, dz.T @ X, dz.sum(0), G)
+    err = (dz_err @ W.abs() + (N + 4) * U * (dz.abs() + dz_err) @ W.abs(), dz_err.T @ X.abs() + (M + 4) * U * (dz.abs() + dz_err).T @ X.abs(),
+           e.sum(0) + (M + 4) * U * (dz.abs() + e).sum(0), torch.zeros_like(G))
+    for name, got, v, b in zip(("x", "weight", "bias", "residual"), grads, want, err):
+        assert bool(torch.isfinite(got).all()), name
+        within(got, v, b + uT * (v.abs() + b) + tiny(dt), f"gradient of {name}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_linear_pre_activation_that_rounds_to_infinity_in_bf16(gpu, act):
+    """-1.998 2^127 is a number in f32 and rounds to -infinity in bf16: the slope there is 0."""
+    import nemo_amd
+    x = torch.full((1, 2), -2.0 ** 64, device=gpu, dtype=torch.bfloat16).requires_grad_()
+    w = torch.tensor([[1.9921875 * 2.0 ** 63, 0.005859375 * 2.0 ** 63]], device=gpu, dtype=torch.bfloat16).requires_grad_()
+    y = nemo_amd.linear(x, w, activation=act)
+    gx, gw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert not y.any() and not gx.any() and not gw.any()
