@@ -2,14 +2,16 @@
 rows with entropy and best alternatives (`log_probs`), and both joined without the [slots, bank rows] matrix (`bank_log_probs`).
 
 The reference computes this loss in torch from FeatureBankNeMo's similarity and MaskCreater's weights (nemo/models/nemo.py:138-209):
-softmax over the bank's rows of similarity / T - weight, cross entropy at the slot's own row.  All functions are differentiable (once),
-run on the current stream of their tensors' device, never synchronise, and raise before any launch on arguments they do not take.
+softmax over the bank's rows of similarity / T - weight, cross entropy at the slot's own row.  All functions are differentiable (once, by a
+backward pass; tensors with forward-mode tangents are refused), run on the current stream of their tensors' device, never synchronise, and raise
+before any launch on arguments they do not take.
 They may be captured into a graph, with their backward pass too; as with torch's own operators no eager autograd graph of the same leaves may
 be alive then (the leaves' gradients would be gathered on the stream of that graph, outside the capture): drop its results first.
 """
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -33,6 +35,13 @@ def _device_tensors(what, dtypes, names, *tensors):
             raise TypeError(f"{what}: {name} is {t.dtype}, {names[0]} {first.dtype}")
 
 
+def _no_tangents(what, *tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0:                  # within forward_ad.dual_level()
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no tangent for forward-mode derivatives (backward passes only)")
+
+
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -46,6 +55,7 @@ def _once(gradients):
     guarded = once_differentiable(gradients)
 
     def backward(ctx, *grads):
+        _no_tangents("backward pass", *grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else gradients(ctx, *grads)
     return backward
 
@@ -112,6 +122,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
         M *= n
     if x.dim() != 2:
         x, residual = x.reshape(M, K), None if residual is None else residual.reshape(M, N)
+    _no_tangents("linear", x, weight, bias, residual)
     if _wants_grad(x, weight, bias, residual):
         y = _Linear.apply(x, weight, bias, residual, activation, alpha, beta)
     else:
@@ -189,6 +200,7 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0):
         raise ValueError(f"log_probs: logits must be [S, V], got {tuple(logits.shape)}")
     S, V = logits.shape
     targets, scale, top = _probs_arguments("log_probs", S, V, logits.device, targets, weights, scale, top)
+    _no_tangents("log_probs", logits, weights)
     if _wants_grad(logits):
         return LogProbs(*_LogProbs.apply(logits, targets, weights, scale, top))
     return LogProbs(*_results(ops.log_probs(logits, targets, weights, scale, top, want_stats=False)))
@@ -229,6 +241,7 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
         raise ValueError(f"bank_log_probs: {features.shape[1]} channels (takes 1 to 256: use linear and log_probs)")
     S, V = features.shape[0], bank.shape[0]
     targets, scale, top = _probs_arguments("bank_log_probs", S, V, features.device, targets, weights, scale, top)
+    _no_tangents("bank_log_probs", features, bank, weights)
     if _wants_grad(features, bank):
         return LogProbs(*_BankLogProbs.apply(features, bank, targets, weights, scale, top))
     return LogProbs(*_results(ops.bank_log_probs(features, bank, targets, weights, scale, top, want_stats=False)))

@@ -71,3 +71,30 @@ def test_linear_pre_activation_that_rounds_to_infinity_in_bf16(gpu, act):
     y = nemo_amd.linear(x, w, activation=act)
     gx, gw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
     assert not y.any() and not gx.any() and not gw.any()
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(gpu):
+    """No tangent is computed: a dual tensor is refused instead of being taken for a constant, with and without gradients."""
+    import nemo_amd
+    from torch.autograd import forward_ad
+    x, w, t = torch.ones(4, 16, device=gpu), torch.ones(9, 16, device=gpu), torch.zeros(4, dtype=torch.int64, device=gpu)
+    weights = torch.zeros(9, device=gpu)
+    bank_logits = lambda v: nemo_amd.linear(v, w)
+    calls = (bank_logits, lambda v: nemo_amd.linear(x, w, residual=torch.ones(4, 9, device=gpu), bias=v[0, :9]), lambda v: nemo_amd.log_probs(v, t),
+             lambda v: nemo_amd.bank_log_probs(v, w, t), lambda v: nemo_amd.log_probs(x, t, weights=v[0]))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                call(dual)
+        assert torch.equal(nemo_amd.linear(x, w), torch.full((4, 9), 16.0, device=gpu))       # ordinary tensors are taken
+        assert not nemo_amd.log_probs(x, t, weights=torch.zeros(16, device=gpu)).logp.isnan().any()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(bank_logits, (x,), (x,))
+    leaf = x.clone().requires_grad_()                                  # a backward pass of a dual gradient
+    for y in (nemo_amd.linear(leaf, w), nemo_amd.log_probs(leaf, t).lse, nemo_amd.bank_log_probs(leaf, w, t).lse):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
