@@ -433,7 +433,7 @@ int nemo_mask_weight(const int32_t* object_idx, const int32_t* source_vert_idx, 
  * may be NULL.  pre [M,N] or NULL: alpha x W^T + bias in the element type, what nemo_linear_backward needs when there is an
  * activation (for all but grad_residual).  K = 0 gives act(bias) + beta residual.  workspace: nemo_linear_workspace bytes of device memory
  * (asked with the same pointers and strides: operands whose rows are not aligned to 16 bytes are copied into it), contents
- * undefined before and after.  Rows of the two operands (and of grad_y below) may lie up to 4 MiB apart, a matrix may have 2^34 elements. */
+ * undefined before and after.  Rows of the two operands may lie up to 4 MiB apart, a matrix may have 2^34 elements. */
 size_t nemo_linear_workspace(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K, int32_t dtype);
 int nemo_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                 int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation, float alpha, float beta, void* y, void* pre,
@@ -442,7 +442,7 @@ int nemo_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
  *   grad_x = alpha dz W, grad_weight = alpha dz^T x, grad_bias = column sums of dz, grad_residual = beta grad_y.
  * Any output may be NULL (not wanted); operands that only unwanted outputs need may be NULL too.  dz is rounded to the
  * element type in front of the two products (they run on the matrix cores); the column sums take it unrounded.  Sums run in a
- * fixed order: two calls give the same bits. */
+ * fixed order: two calls give the same bits.  grad_x and grad_weight take rows of grad_y up to 4 MiB long, as far apart as they may be. */
 size_t nemo_linear_backward_workspace(const void* grad_y, int64_t ldg, const void* x, int64_t ldx, const void* weight, int64_t ldw,
                                       int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation);
 int nemo_linear_backward(const void* grad_y, int64_t ldg, const void* x, int64_t ldx, const void* weight, int64_t ldw,

@@ -104,7 +104,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     x [..., K], weight [N, K], bias [N], residual [..., N] of one type (float32, bfloat16 or float16) -> [..., N] of that type.
     activation: "none", "relu", "gelu" (the exact one, with erf) or "silu".  Products are summed in 32 bits (float32: on the f32 matrix
     cores, so infinities and NaN come out as in any f32 product) and the result is rounded once.  x, weight, bias and residual are
-    differentiable.  Rows of x, weight and residual may be strided; alignment matters for speed only.  Rows of x and weight take up to 4 MiB."""
+    differentiable.  Rows of x, weight and residual may be strided; alignment matters for speed only.  Rows of x and weight take
+    up to 4 MiB, and so do rows of the result where x or weight gets a gradient."""
     _device_tensors("linear", ops.DTYPES, ("x", "weight", "bias", "residual"), x, weight, bias, residual)
     if activation not in ops.ACTIVATIONS:
         raise ValueError(f"linear: activation {activation!r} (takes {', '.join(ops.ACTIVATIONS)})")
@@ -124,6 +125,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
         x, residual = x.reshape(M, K), None if residual is None else residual.reshape(M, N)
     _no_tangents("linear", x, weight, bias, residual)
     if _wants_grad(x, weight, bias, residual):
+        if M and K and N * x.element_size() > 1 << 22 and _wants_grad(x, weight):       # what the backward pass takes
+            raise ValueError(f"linear: rows of {N} results, more than 4 MiB, with gradients of x or weight")
         y = _Linear.apply(x, weight, bias, residual, activation, alpha, beta)
     else:
         y, _ = ops.linear(x, weight, bias, residual, activation, alpha, beta)

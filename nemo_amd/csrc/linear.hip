@@ -663,10 +663,11 @@ static int check_linear(const char* who, int64_t M, int64_t N, int64_t K, int dt
     return NEMO_OK;
 }
 
-// Offsets within a tile of 256 rows are 32-bit.  cols: the contiguous extent, what a packed copy has.
+// Offsets within a tile of 256 rows are 32-bit: rows lie at most 4 MiB apart.  cols: the contiguous extent, what a packed copy has.
+constexpr int64_t kRowBytes = 1 << 22;
 static int check_stride(const char* who, const void* p, int64_t ld, int64_t cols, int dtype) {
     const int es = elem_size(dtype);
-    if ((ready(p, ld, cols, es) ? ld : pad16(cols, es)) * es > (1 << 22)) return fail(NEMO_ERR_UNSUPPORTED, "%s: rows more than 4 MiB apart", who);
+    if ((ready(p, ld, cols, es) ? ld : pad16(cols, es)) * es > kRowBytes) return fail(NEMO_ERR_UNSUPPORTED, "%s: rows more than 4 MiB apart", who);
     return NEMO_OK;
 }
 
@@ -710,9 +711,9 @@ extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64
     return NEMO_OK;
 }
 
-// dz is the incoming gradient itself where there is no activation and its rows suit the tiles.
+// dz is the incoming gradient itself where there is no activation and its rows suit the tiles; else it is written with padded rows.
 static bool slope_needed(const void* grad_y, int64_t ldg, int64_t N, int dtype, int act) {
-    return act != ACT_NONE || !ready(grad_y, ldg, N, elem_size(dtype));
+    return act != ACT_NONE || !ready(grad_y, ldg, N, elem_size(dtype)) || ldg * elem_size(dtype) > kRowBytes;
 }
 
 extern "C" size_t nemo_linear_backward_workspace(const void* grad_y, int64_t ldg, const void* x, int64_t ldx, const void* weight, int64_t ldw,
@@ -757,7 +758,9 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
     if (M > 0 && N > 0 && K > 0 && ((grad_x && (!weight || ldw < K)) || (grad_weight && (!x || ldx < K))))
         return fail(NEMO_ERR_INVALID, "nemo_linear_backward: null operand or a row stride shorter than the row");
     if (M > 0 && N > 0 && K > 0 && (grad_x || grad_weight)) {
-        if ((rc = check_stride("nemo_linear_backward", grad_y, ldg, N, dtype)) || (grad_x && (rc = check_stride("nemo_linear_backward", weight, ldw, K, dtype))) ||
+        if (pad16(N, elem_size(dtype)) * (int64_t)elem_size(dtype) > kRowBytes)
+            return fail(NEMO_ERR_UNSUPPORTED, "nemo_linear_backward: rows of grad_y longer than 4 MiB");
+        if ((grad_x && (rc = check_stride("nemo_linear_backward", weight, ldw, K, dtype))) ||
             (grad_weight && (rc = check_stride("nemo_linear_backward", x, ldx, K, dtype))))
             return rc;
     }

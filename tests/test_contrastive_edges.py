@@ -1,4 +1,6 @@
 """The contrastive loss's operators where sizes, values and strides leave the ordinary range; tolerances as in test_contrastive.py."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -98,3 +100,50 @@ def test_forward_mode_is_refused(gpu):
     for y in (nemo_amd.linear(leaf, w), nemo_amd.log_probs(leaf, t).lse, nemo_amd.bank_log_probs(leaf, w, t).lse):
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.gpu
+def test_linear_rows_of_results_beyond_the_backward_pass(gpu):
+    """Results of more than 4 MiB a row: taken without gradients of x and weight, refused with them before anything runs."""
+    import nemo_amd
+    N = (1 << 20) + 8
+    x, w, b = torch.ones(2, 4, device=gpu), torch.ones(N, 4, device=gpu), torch.zeros(N, device=gpu)
+    assert bool((nemo_amd.linear(x, w, b) == 4.0).all())
+    for leaf in (x, w):
+        leaf.requires_grad_()
+        with pytest.raises(ValueError, match="4 MiB"):
+            nemo_amd.linear(x, w, b)
+        leaf.requires_grad_(False)
+    y = nemo_amd.linear(x, w, b.requires_grad_())
+    (gb,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    assert bool((gb == 2.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_gradient_with_rows_far_apart(gpu, dtype):
+    """An incoming gradient that is a slice of rows more than 4 MiB long."""
+    import nemo_amd
+    dt = TYPES[dtype]
+    gen = torch.Generator(device=gpu).manual_seed(2)
+    x, w = (torch.randn(n, 40, generator=gen, device=gpu).to(dt).requires_grad_() for n in (5, 64))
+    wide = torch.randn(5, (1 << 21) + 64, generator=gen, device=gpu).to(dt)
+    y = nemo_amd.linear(x, w)
+    for g in (wide[:, :64], wide[:, 1:65]):
+        got = torch.autograd.grad(y, (x, w), g, retain_graph=True)
+        want = torch.autograd.grad(y, (x, w), g.contiguous(), retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_entry_takes_gradients_with_rows_far_apart():
+    """The C entry asks for a copy of such rows instead of refusing them; a row itself may be no longer than 4 MiB."""
+    from tests.test_contrastive import _lib_or_skip
+    lib = _lib_or_skip()
+    p = C.c_void_p(4096)
+    near, far = (lib.nemo_linear_backward_workspace(p, ld, p, 8, p, 8, 4, 8, 8, 0, 0) for ld in (8, (1 << 20) + 4))
+    assert far == near + 256                                           # 4 rows of 32 bytes, in whole 256s
+
+    def backward(ldg, N):
+        return lib.nemo_linear_backward(p, ldg, p, 8, p, 8, None, 4, N, 8, 0, 0, 1.0, 1.0, p, p, None, None, None, 0, None)
+    assert backward((1 << 20) + 4, 8) == -1 and "workspace" in lib.nemo_last_error().decode()
+    assert backward((1 << 20) + 4, (1 << 20) + 4) == -2 and "4 MiB" in lib.nemo_last_error().decode()
