@@ -486,7 +486,7 @@ int nemo_bank_log_probs(const void* features, int64_t ldf, const void* bank, int
 /* With dz as nemo_log_probs_backward has it (without its factor scale):
  *   grad_features[i] = scale sum_j dz[i,j] bank[j],   grad_bank[j] = scale sum_i dz[i,j] features[i]
  * (contiguous, element type dtype; NULL: not wanted).  weights, scale and top as in the call that wrote `stats` (they decide the form in
- * which it is kept).  The scores are computed again.  Places that are left out add nothing, whatever the
+ * which it is kept); rows of weights at most 2^27 elements apart.  The scores are computed again.  Places that are left out add nothing, whatever the
  * feature or bank row holds.  Rows whose target is outside -1..cols-1 make grad_features[i] and all of grad_bank NaN.  bf16: dz is
  * multiplied as two bf16 pieces, f32: as three.  Sums run in a fixed order: two calls give the same bits. */
 size_t nemo_bank_log_probs_backward_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,

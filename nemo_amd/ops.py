@@ -704,9 +704,12 @@ def _on(device):
     return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def rows_2d(t, width):
+_FAR_BYTES, _FAR_WEIGHTS = 1 << 22, 1 << 27           # how far apart rows of linear's operands (bytes) and of the bank's weights (elements) may lie
+
+
+def rows_2d(t, width, apart=None):
     """(t as [rows, width] whose rows are contiguous, row stride in elements): a view where the strides allow it, else a copy.
-    Rows may lie apart (a slice of wider rows); overlapping or permuted ones are copied."""
+    Rows may lie apart (a slice of wider rows), up to `apart` elements; overlapping or permuted ones are copied."""
     if t.dim() != 2:
         rows = 1
         for n in t.shape[:-1]:
@@ -716,7 +719,7 @@ def rows_2d(t, width):
         return t, width
     if t.numel() == 0:
         return t, width
-    if (width == 1 or t.stride(1) == 1) and t.stride(0) >= width:
+    if (width == 1 or t.stride(1) == 1) and t.stride(0) >= width and (apart is None or t.stride(0) <= apart):
         return t, t.stride(0)
     return t.detach().contiguous(), width
 
@@ -740,8 +743,9 @@ def linear(x, weight, bias=None, residual=None, activation="none", alpha=1.0, be
     """-> (y [M,N], pre [M,N] or None): y = act(alpha x weight^T + bias) + beta residual; x [M,K], weight [N,K] of one type."""
     lib = _lib.load()
     (M, K), N = x.shape, weight.shape[0]
-    x, ldx = rows_2d(x, K)
-    weight, ldw = rows_2d(weight, K)
+    apart = _FAR_BYTES // x.element_size()
+    x, ldx = rows_2d(x, K, apart)
+    weight, ldw = rows_2d(weight, K, apart)
     ldr = N
     if residual is not None:
         residual, ldr = rows_2d(residual, N)
@@ -764,8 +768,9 @@ def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1
     for grad_x: either may be its shape instead."""
     lib = _lib.load()
     (M, K), (N, _) = (t.shape if torch.is_tensor(t) else t for t in (x, weight))
-    x, ldx = rows_2d(x, K) if torch.is_tensor(x) else (None, K)
-    weight, ldw = rows_2d(weight, K) if torch.is_tensor(weight) else (None, K)
+    apart = _FAR_BYTES // grad_y.element_size()
+    x, ldx = rows_2d(x, K, apart) if torch.is_tensor(x) else (None, K)
+    weight, ldw = rows_2d(weight, K, apart) if torch.is_tensor(weight) else (None, K)
     grad_y, ldg = rows_2d(grad_y, N)
     dev, dt = grad_y.device, DTYPES[grad_y.dtype]
     shapes = ((M, K), (N, K), (N,), (M, N))
@@ -780,7 +785,7 @@ def linear_backward(grad_y, x, weight, pre, activation="none", alpha=1.0, beta=1
     return tuple(outs)
 
 
-def _row_weights(weights, cols):
+def _row_weights(weights, cols, apart=None):
     """(tensor, row stride) of log-prob weights: None, one row for all ([cols], stride 0) or a row each."""
     if weights is None:
         return None, 0
@@ -788,7 +793,7 @@ def _row_weights(weights, cols):
         weights = weights[0]                                                # one row expanded
     if weights.dim() == 1:
         return weights.contiguous(), 0
-    return rows_2d(weights, cols)
+    return rows_2d(weights, cols, apart)
 
 
 def _f32_row(g):
@@ -850,7 +855,7 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0, want
     (S, ch), V = features.shape, bank.shape[0]
     features, ldf = rows_2d(features, ch)
     bank, ldb = rows_2d(bank, ch)
-    weights, ldw = _row_weights(weights, V)
+    weights, ldw = _row_weights(weights, V, _FAR_WEIGHTS)
     targets = targets.contiguous()
     dev, dt = features.device, DTYPES[features.dtype]
     out = _Probs(S, top, want_stats, dev)
@@ -869,7 +874,7 @@ def bank_log_probs_backward(features, bank, targets, weights, stats, g_logp, g_e
     (S, ch), V = features.shape, bank.shape[0]
     features, ldf = rows_2d(features, ch)
     bank, ldb = rows_2d(bank, ch)
-    weights, ldw = _row_weights(weights, V)
+    weights, ldw = _row_weights(weights, V, _FAR_WEIGHTS)
     targets = targets.contiguous()
     dev, dt = features.device, DTYPES[features.dtype]
     gs = [_f32_row(g) for g in (g_logp, g_entropy, g_lse)]

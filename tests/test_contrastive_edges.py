@@ -147,3 +147,36 @@ def test_entry_takes_gradients_with_rows_far_apart():
         return lib.nemo_linear_backward(p, ldg, p, 8, p, 8, None, 4, N, 8, 0, 0, 1.0, 1.0, p, p, None, None, None, 0, None)
     assert backward((1 << 20) + 4, 8) == -1 and "workspace" in lib.nemo_last_error().decode()
     assert backward((1 << 20) + 4, (1 << 20) + 4) == -2 and "4 MiB" in lib.nemo_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bank_weights_with_rows_far_apart(gpu, dtype):
+    """Rows of weights more than 2^27 elements apart, forward and backward."""
+    import nemo_amd
+    gen = torch.Generator(device=gpu).manual_seed(2)
+    f, b = (torch.randn(n, 32, generator=gen, device=gpu).to(TYPES[dtype]).requires_grad_() for n in (3, 70))
+    t = torch.tensor([0, 69, -1], device=gpu)
+    far = torch.zeros(2 * ((1 << 27) + 8) + 70, device=gpu).as_strided((3, 70), ((1 << 27) + 8, 1))
+    far.copy_(torch.rand(3, 70, generator=gen, device=gpu))
+    out = []
+    for weights in (far, far.contiguous()):
+        r = nemo_amd.bank_log_probs(f, b, t, weights, scale=0.2, top=2)
+        out.append([*r, *torch.autograd.grad((r.logp + r.entropy).sum(), (f, b))])
+    assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_operands_with_rows_far_apart(gpu, dtype):
+    """Slices of rows more than 4 MiB long, on 16 bytes and off them."""
+    import nemo_amd
+    dt = TYPES[dtype]
+    gen = torch.Generator(device=gpu).manual_seed(2)
+    wide = torch.randn(5, (1 << 21) + 64, generator=gen, device=gpu).to(dt)
+    for x, w in ((wide[:, :40], wide[:3, 64:104]), (wide[:, 1:41], wide[:3, 3:43])):
+        out = []
+        for leaves in ([x.detach().requires_grad_(), w.detach().requires_grad_()], [t.contiguous().requires_grad_() for t in (x, w)]):
+            y = nemo_amd.linear(*leaves, activation="silu")
+            out.append([y, *torch.autograd.grad(y.sum(), leaves)])
+        assert all(torch.equal(p, q) for p, q in zip(*out))
