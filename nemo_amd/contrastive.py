@@ -3,8 +3,9 @@ rows with entropy and best alternatives (`log_probs`), and both joined without t
 
 The reference computes this loss in torch from FeatureBankNeMo's similarity and MaskCreater's weights (nemo/models/nemo.py:138-209):
 softmax over the bank's rows of similarity / T - weight, cross entropy at the slot's own row.  All functions are differentiable (once, by a
-backward pass; tensors with forward-mode tangents are refused), run on the current stream of their tensors' device, never synchronise, and raise
-before any launch on arguments they do not take.
+backward pass; tensors with forward-mode tangents are refused), run on the current stream of their tensors' device, and raise before any launch on
+arguments they do not take.  They never synchronise on device tensors; targets on the host are checked there and copied, which waits for the
+stream and is refused while it is captured.
 They may be captured into a graph, with their backward pass too; as with torch's own operators no eager autograd graph of the same leaves may
 be alive then (the leaves' gradients would be gathered on the stream of that graph, outside the capture): drop its results first.
 """
@@ -145,6 +146,8 @@ def _probs_arguments(what, rows, cols, device, targets, weights, scale, top):
     if targets.device != device:
         if targets.is_cuda:
             raise RuntimeError(f"{what}: targets are on {targets.device}, the rows on {device}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what}: targets are on the host, a capture takes none (the copy waits for the stream): copy them to the device before")
         if targets.numel() and (int(targets.min()) < -1 or int(targets.max()) >= cols):      # on the host: nothing to wait for
             raise ValueError(f"{what}: targets must lie in -1 .. {cols - 1}")
     if weights is not None:
@@ -195,7 +198,7 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0):
 
     targets [S] int64 or int32: the place, or -1 for a row without a target (logp 0, no gradient through it).  Other values outside the row
     are refused where the tensor is on the host and give NaN in that row (values and gradient) where it is on the device, which is not read
-    back.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place out, whatever the logit there is (NaN
+    back.  Targets on the host cost a blocking copy.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place out, whatever the logit there is (NaN
     too).  A row with nothing left: lse and logp -inf, entropy 0, top_index -1, gradient 0.  A row with a NaN or +inf left: NaN,
     top_index -1.  Fewer places left than `top`: -inf and -1 in their stead."""
     _device_tensors("log_probs", ops.DTYPES, ("logits",), logits)

@@ -180,3 +180,24 @@ def test_linear_operands_with_rows_far_apart(gpu, dtype):
             y = nemo_amd.linear(*leaves, activation="silu")
             out.append([y, *torch.autograd.grad(y.sum(), leaves)])
         assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+@pytest.mark.gpu
+def test_host_targets_in_a_capture(gpu):
+    """Targets on the host are copied with a blocking copy, which a capture does not take: refused, and the capture goes on."""
+    import nemo_amd
+    x, w, t = torch.randn(4, 16, device=gpu), torch.randn(9, 16, device=gpu), torch.zeros(4, dtype=torch.int64)
+    eager = nemo_amd.log_probs(x, t).lse
+    assert torch.equal(eager, nemo_amd.log_probs(x, t.to(gpu)).lse)
+    t_dev = t.to(gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: nemo_amd.log_probs(x, t), lambda: nemo_amd.bank_log_probs(x, w, t)):
+            with pytest.raises(RuntimeError, match="on the host"):
+                call()
+        lse = nemo_amd.log_probs(x, t_dev).lse
+    for _ in range(3):
+        lse.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(lse, eager)
