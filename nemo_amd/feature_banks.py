@@ -180,7 +180,12 @@ class FeatureBankNeMo(nn.Module):
     # ---- the contrastive loss ----
     def logits(self, feats, weights=None, T=1.0):
         """similarity / T - weights of slots [S, C] with every bank row, [S, V_total + clutter rows], differentiable with respect to the
-        slots (and to weights): the logits of the reference's cross entropy.  weights: MaskCreater's rows, in the slots' type, or None."""
+        slots (and to weights): the logits of the reference's cross entropy.  weights: MaskCreater's rows, one row for all slots, or
+        None; they are rounded to the slots' type, that of the result (in float16 a weight beyond 65504 leaves its place out)."""
+        if weights is not None:
+            weights = weights.to(feats.dtype)
+            if weights.dim() == 1:
+                weights = weights.expand(*feats.shape[:-1], -1)
         return contrastive.linear(feats, self.memory.to(feats.dtype), residual=weights, alpha=1.0 / T, beta=-1.0)
 
     def log_probs(self, feats, rows, weights=None, T=1.0, top=0):

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_contrastive import ACT, CURVE, INF, TYPES, U, bank_case, half_step, tiny, within
+from tests.test_contrastive import ACT, CURVE, INF, TYPES, U, bank_case, half_step, loss_case, tiny, within
 
 
 @pytest.mark.gpu
@@ -201,3 +201,30 @@ def test_host_targets_in_a_capture(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(lse, eager)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_bank_logits_take_the_weights_of_log_probs(gpu, dtype):
+    """MaskCreater's f32 weights with slots of any type.  They are rounded to the slots' type (a weight beyond f16 leaves its place out), the result
+    once more."""
+    dt = TYPES[dtype]
+    bank, x, visible, _, weights, rows = loss_case(gpu, True)
+    slots = x[:, :visible.shape[1]][visible].to(dt)
+    weights = weights + 0.3 * (torch.arange(weights.shape[1], device=gpu) % 3)
+    T = 0.07
+    leaf = weights.clone().requires_grad_()
+    got = bank.logits(slots, leaf, T)
+    assert got.dtype == dt
+    w = weights.to(dt).double()
+    S, B = slots.double(), bank.memory.to(dt).double()
+    want = S @ B.T / T - w
+    err = 2 * (32 + 8) * U / T * (S.abs() @ B.abs().T) + 4 * U * want.abs()
+    want_t = torch.where(want.abs() > torch.finfo(dt).max, torch.sign(want) * INF, want)
+    within(got, want_t, torch.nan_to_num(err + half_step(dt) * (want.abs() + err), 0, 0, 0), "logits")
+    (gw,) = torch.autograd.grad(got, leaf, torch.ones_like(got))
+    assert gw.dtype == torch.float32 and bool((gw == -1.0).all())
+    assert torch.equal(bank.logits(slots, weights.to(dt), T), got.detach())
+    assert torch.equal(bank.logits(slots, weights[0], T), bank.logits(slots, weights[:1].expand_as(weights), T))
+    r = bank.log_probs(slots, rows, weights, T)
+    assert bool(torch.isfinite(r.logp).all())
