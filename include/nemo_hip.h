@@ -474,7 +474,8 @@ int nemo_log_probs_backward(const void* logits, int64_t ld, const float* weights
 /* nemo_log_probs straight from features [rows,channels] and bank [cols,channels] (f32 or bf16, both the same):
  *   z[i,j] = scale <features[i], bank[j]> - weights[i,j],
  * same outputs and rules, the [rows,cols] matrix is never written.  Products are summed in f32.  f32 rows are multiplied as three bf16 pieces
- * (24 bits together, as exact as f32 products; an infinity in a row makes its scores NaN, whatever its sign).  channels 1..256 (padded to 64,
+ * (24 bits together, as exact as f32 products; an infinity in a row makes its scores NaN, whatever its sign).  Without
+ * weights and with top = 0 scores are summed in units of log 2, those beyond 2.3e38 count as infinities.  channels 1..256 (padded to 64,
  * 128 or 256); rows and cols below 2^24.  workspace: nemo_bank_log_probs_workspace bytes asked with the same pointers and strides
  * (pieces, and rows that do not start on 16 bytes, are written into it), contents undefined before and after. */
 size_t nemo_bank_log_probs_workspace(const void* features, int64_t ldf, const void* bank, int64_t ldb, int64_t rows, int64_t cols,

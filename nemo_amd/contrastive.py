@@ -65,8 +65,8 @@ def _number(what, name, value):
     if torch.is_tensor(value):
         raise TypeError(f"{what}: {name} must be a number, not a tensor (it is read on the host and has no gradient)")
     value = float(value)
-    if value != value or value in (float("inf"), -float("inf")):
-        raise ValueError(f"{what}: {name} must be finite, got {value}")
+    if not abs(value) <= 3.4028234663852886e38:
+        raise ValueError(f"{what}: {name} must be finite in 32 bits, got {value}")
     return value
 
 
@@ -198,9 +198,9 @@ def log_probs(logits, targets, weights=None, scale=1.0, top=0):
 
     targets [S] int64 or int32: the place, or -1 for a row without a target (logp 0, no gradient through it).  Other values outside the row
     are refused where the tensor is on the host and give NaN in that row (values and gradient) where it is on the device, which is not read
-    back.  Targets on the host cost a blocking copy.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place out, whatever the logit there is (NaN
-    too).  A row with nothing left: lse and logp -inf, entropy 0, top_index -1, gradient 0.  A row with a NaN or +inf left: NaN,
-    top_index -1.  Fewer places left than `top`: -inf and -1 in their stead."""
+    back.  Targets on the host cost a blocking copy.  weights float32, [V] for all rows or [S, V]: subtracted constants; +inf leaves the place
+    out, whatever the logit there is (NaN too).  A row with nothing left: lse and logp -inf, entropy 0, top_index -1, gradient 0.  A row with a
+    NaN or +inf left: NaN, top_index -1.  Fewer places left than `top`: -inf and -1 in their stead."""
     _device_tensors("log_probs", ops.DTYPES, ("logits",), logits)
     if logits.dim() != 2:
         raise ValueError(f"log_probs: logits must be [S, V], got {tuple(logits.shape)}")
@@ -238,8 +238,9 @@ def bank_log_probs(features, bank, targets, weights=None, scale=1.0, top=0):
     """log_probs(linear(features, bank), ...) without the [S, V] matrix: features [S, C] and bank [V, C], both float32 or both bfloat16, C up
     to 256, S and V below 2^24.  Scores are z = scale <feature, bank row> - weights, summed in 32 bits; arguments, results and rules are
     those of log_probs.  float32 rows are multiplied as three bfloat16 pieces (24 bits together): products are as exact as float32's, but
-    an infinity in a row makes its scores NaN, whatever its sign.  Differentiable with respect to features and bank; the gradient computes
-    the scores again instead of keeping them; it may be split in another way than the values, and two calls give the same bits."""
+    an infinity in a row makes its scores NaN, whatever its sign.  Without weights and `top` scores beyond 2.3e38 count as infinities.
+    Differentiable with respect to features and bank; the gradient computes the scores again instead of keeping them; it may be split in
+    another way than the values, and two calls give the same bits."""
     _device_tensors("bank_log_probs", (torch.float32, torch.bfloat16), ("features", "bank"), features, bank)
     if features.dim() != 2 or bank.dim() != 2 or features.shape[1] != bank.shape[1]:
         raise ValueError(f"bank_log_probs: features must be [S, C] and bank [V, C], got {tuple(features.shape)} and {tuple(bank.shape)}")

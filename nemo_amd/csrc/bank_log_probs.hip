@@ -127,10 +127,11 @@ static Parts gradient_parts(int64_t owners, int64_t others, int cp, int dtype) {
     return parts_of_bank(owners, others, dtype == NEMO_F32 ? (cp == 64 ? 2 : 1) : cp <= 128 ? 2 : 1, 2);
 }
 
-// The state's form: 0 where it is kept of the scores, else what turns a product into its score in units of log 2.
+// The state's form: 0 where it is kept of the scores, else what turns a product into its score in units of log 2 (with hardly any scale it would be
+// inexact, with the largest ones infinite).
 static float product_unit(const float* weights, float scale, int top) {
     const float s = scale < 0.0f ? -scale : scale;
-    return weights || top > 0 || !(s >= 1.0e-30f) ? 0.0f : s * kLog2e;
+    return weights || top > 0 || !(s >= 1.0e-30f && s <= 1.0e30f) ? 0.0f : s * kLog2e;
 }
 
 static int check_bank(const char* who, int64_t rows, int64_t cols, int64_t channels, int dtype, int top) {

@@ -228,3 +228,20 @@ def test_bank_logits_take_the_weights_of_log_probs(gpu, dtype):
     assert torch.equal(bank.logits(slots, weights[0], T), bank.logits(slots, weights[:1].expand_as(weights), T))
     r = bank.log_probs(slots, rows, weights, T)
     assert bool(torch.isfinite(r.logp).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bank_scale_near_the_largest_number(gpu, dtype):
+    """scale log2 e is beyond f32: products of 0 and of 2^-126 give scores of 0 and 3.5."""
+    f, b = (torch.eye(n, 64, device=gpu).mul_(2.0 ** -63).to(TYPES[dtype]) for n in (64, 50))
+    for scale in (3.0e38, -3.0e38):
+        bank_case(gpu, 64, 50, 64, TYPES[dtype], "none", 0, scale=scale, features=f, bank=b)
+
+
+def test_numbers_beyond_f32_are_refused():
+    from nemo_amd import contrastive
+    for v in (1e39, -1e39, 3.4028236e38):
+        with pytest.raises(ValueError, match="finite"):
+            contrastive._number("linear", "alpha", v)
+    assert contrastive._number("linear", "alpha", 3.4028234663852886e38) == 3.4028234663852886e38
