@@ -424,7 +424,8 @@ int nemo_mask_weight(const int32_t* object_idx, const int32_t* source_vert_idx, 
  * The loss over the bank (softmax of similarity / T - weight over the bank's rows, cross entropy at the slot's own row:
  * what the reference's training step computes from FeatureBankNeMo's similarity and MaskCreater's weights,
  * nemo/models/nemo.py:138-209, nemo/models/feature_banks.py:39-232) and the dense layer in front of it.  Rows may be
- * strided (a row stride `ld*` in elements, elements of a row contiguous); outputs are contiguous.  Element types: */
+ * strided (a row stride `ld*` in elements, elements of a row contiguous); outputs are contiguous.  Workspaces start on 16 bytes.
+ * Element types: */
 #define NEMO_F32  0
 #define NEMO_BF16 1
 #define NEMO_F16  2

@@ -192,6 +192,7 @@ extern "C" int nemo_bank_log_probs(const void* features, int64_t ldf, const void
     const size_t need = nemo_bank_log_probs_workspace(features, ldf, bank, ldb, rows, cols, channels, dtype, top);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && ((uintptr_t)workspace & 15)) return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs: the workspace must start on 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     RowsIn f, b;
@@ -243,6 +244,7 @@ extern "C" int nemo_bank_log_probs_backward(const void* features, int64_t ldf, c
     const size_t need = nemo_bank_log_probs_backward_workspace(features, ldf, bank, ldb, rows, cols, channels, dtype);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && ((uintptr_t)workspace & 15)) return fail(NEMO_ERR_INVALID, "nemo_bank_log_probs_backward: the workspace must start on 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     const float unit = product_unit(weights, scale, top);

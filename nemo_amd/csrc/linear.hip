@@ -694,6 +694,7 @@ extern "C" int nemo_linear(const void* x, int64_t ldx, const void* weight, int64
     const size_t need = nemo_linear_workspace(x, ldx, weight, ldw, M, N, K, dtype);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && ((uintptr_t)workspace & 15)) return fail(NEMO_ERR_INVALID, "nemo_linear: the workspace must start on 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     Operand P = {weight, ldw}, Q = {x, ldx};
@@ -767,6 +768,7 @@ extern "C" int nemo_linear_backward(const void* grad_y, int64_t ldg, const void*
     const size_t need = nemo_linear_backward_workspace(grad_y, ldg, x, ldx, weight, ldw, M, N, K, dtype, activation);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && ((uintptr_t)workspace & 15)) return fail(NEMO_ERR_INVALID, "nemo_linear_backward: the workspace must start on 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     const int es = elem_size(dtype);
     char* ws = (char*)workspace;

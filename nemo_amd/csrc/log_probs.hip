@@ -356,6 +356,7 @@ extern "C" int nemo_log_probs(const void* logits, int64_t ld, const float* weigh
     const size_t need = nemo_log_probs_workspace(rows, cols, top);
     if (workspace_bytes < need || (need && !workspace))
         return fail(NEMO_ERR_INVALID, "nemo_log_probs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && ((uintptr_t)workspace & 15)) return fail(NEMO_ERR_INVALID, "nemo_log_probs: the workspace must start on 16 bytes");
     LogProbArgs a = {};
     a.logits = logits; a.ld = ld; a.weights = weights; a.ldw = ldw; a.targets = (const long long*)targets;
     a.rows = rows; a.cols = (int)cols; a.scale = scale;

@@ -245,3 +245,15 @@ def test_numbers_beyond_f32_are_refused():
         with pytest.raises(ValueError, match="finite"):
             contrastive._number("linear", "alpha", v)
     assert contrastive._number("linear", "alpha", 3.4028234663852886e38) == 3.4028234663852886e38
+
+
+def test_entries_refuse_workspaces_off_16_bytes():
+    from tests.test_contrastive import _lib_or_skip
+    lib = _lib_or_skip()
+    p, ws, n = C.c_void_p(4096), C.c_void_p(4104), 1 << 30
+    for rc in (lib.nemo_linear(p, 7, p, 7, None, None, 0, 4, 4, 7, 0, 0, 1.0, 1.0, p, None, ws, n, None),
+               lib.nemo_linear_backward(p, 8, p, 7, p, 7, None, 4, 8, 7, 0, 0, 1.0, 1.0, p, p, None, None, ws, n, None),
+               lib.nemo_log_probs(p, 1 << 20, None, 0, p, 1, 1 << 20, 0, 1.0, 0, p, None, None, None, None, None, ws, n, None),
+               lib.nemo_bank_log_probs(p, 16, p, 16, None, 0, p, 4, 9, 16, 0, 1.0, 0, p, None, None, None, None, None, ws, n, None),
+               lib.nemo_bank_log_probs_backward(p, 16, p, 16, None, 0, p, p, None, None, None, 4, 9, 16, 0, 1.0, 0, p, p, ws, n, None)):
+        assert rc == -1 and "16 bytes" in lib.nemo_last_error().decode()
