@@ -16,8 +16,9 @@
 
 namespace nemo {
 
-// dz of one score or product without the target's share.  In bf16 and without weights m holds m + log2 s, one operation less: off by u |lse|
-// (1e-6 at 16), far below the rounding of dz's pieces.  SAFE: log2 p may be -inf.
+// dz of one score or product without the target's share.  In bf16 and without weights m holds m + log2 s, one operation less: log2 p off by u |lse| /
+// log 2 more, as much as the sums behind a score of that size are off themselves, and below the rounding of dz's pieces up to |lse| of
+// about 100.  SAFE: log2 p may be -inf.
 template <bool F32, bool GENERAL, bool SAFE>
 __device__ inline float pair_gradient(float v, float k, float m, float log2_s, float c, float g2) {
     float lp2;
@@ -104,7 +105,8 @@ __device__ inline void second_product(f32x16_t (&acc)[CP / 32], const char* lds,
 // Measured (features' gradient / bank's gradient, us).  32768 x 15976 x 128 bf16: 335 / 380; the three products of a pair take 303; the bank's reads
 // what dz needs of every feature row from LDS, with which LDS (2.0 k cycles a step of eight waves) is busier than the matrix cores (1.5 k).
 // 10007 x 3678 x 128 f32: 109 / 117, with weights for every pair 125 / 147; the twelve products of a pair take 85.  Weights loaded a
-// step ahead, in 16 more registers, changed nothing (128 / 152).
+// step ahead, in 16 more registers, changed nothing (128 / 152): the compiler waits for all loads under way at the first transposing read of a
+// step, for those too.  It is also why four tiles hide no more of a copy than part of a step.
 //
 // Products of places that are left out must not count even where a feature or bank row holds infinities or NaN (0 x NaN): when a wave ends with
 // a value that is not finite, its workgroup goes through its part again, step after step, with such values of the second product's first

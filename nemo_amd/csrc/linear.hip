@@ -18,11 +18,11 @@
 // The copies to LDS need operands that start on 16 bytes, with rows that do and a contiguous extent of whole 16 bytes; others are first copied into
 // the workspace with padded rows (pack_kernel).  Bias, residual and results may start at any element.
 //
-// Measured (a call).  8192 x 4096 x 4096 bf16 with gelu, bias and residual: 255 us, 1078 TF; the bare product of a library 207 us, 1326 TF.
-// 160000 x 128 x 2048 bf16 with relu and bias (696 MB): 177 us, 3.9 TB/s.  5590 x 15976 x 128 f32 with a residual: 268 us, 86 TF and 2.7 TB/s:
+// Measured (a call).  8192 x 4096 x 4096 bf16 with gelu, bias and residual: 261 us, 1053 TF; the bare product of a library 207 us, 1326 TF.
+// 160000 x 128 x 2048 bf16 with relu and bias (696 MB): 188 us, 3.7 TB/s.  5590 x 15976 x 128 f32 with a residual: 267 us, 86 TF and 2.7 TB/s:
 // the f32 matrix instructions alone take 149 us, reading and writing the 714 MB alone 150, and little of the two overlaps.
-// 8191 x 1001 x 515 f16, rows off 16 bytes, silu, bias, residual: packing 6, product 33 us; backward: packing 6, slope 20, column sums 5,
-// products 24 and 22 + 6 (join).
+// 8191 x 1001 x 515 f16, rows off 16 bytes, silu, bias, residual: packing 6, product 31 us; backward: packing 6, slope 20, column sums 4,
+// products 23 and 20 + 6 (join).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -224,7 +224,9 @@ __device__ inline u32x4 fragment(const char* lds, int row, int kf, int lane) {
 
 // The tile of a step is multiplied in two halves of its k.  Both halves' fragments are in registers before the barrier that frees the tile's
 // buffer; behind it, while the second half is multiplied, the tile after the next one is copied into that buffer and the first half of the
-// next tile is read.  So the matrix cores have work across the barrier, and a copy has a whole step to arrive.
+// next tile is read.  So the matrix cores have work across the barrier, and a copy could have a whole step to arrive.  As compiled it has that in
+// every other step only: the compiler does not tell the two buffers apart.  In the 16-bit forms it waits for the copies just made before it
+// reads the other buffer; in the f32 forms it moves them down to the next barrier, which waits for them.
 template <typename T, int BP, int BQ, int WP, int WQ, bool PT, bool QT>
 __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 1 : BQ == 128 ? 2 : BQ == 64 ? 3 : 4) void gemm_kernel(GemmArgs a) {
     typedef Mma<T> M;
@@ -435,8 +437,10 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob first, PackJob second
     *(typename Loose<T, E>::V*)((T*)j.dst + (long)r * j.ld_out + c) = v;
 }
 
-// dz = dy act'(pre) (rounded to T because the matrix cores take T), dr = beta dy, and per block of rows the column sums of the unrounded
-// dz (for the bias).  A workgroup takes 256 columns x kSlopeRows rows: 32 threads of eight columns, eight rows at a time.  Bound by the latency of
+// dz = dy act'(pre), dr = beta dy, and per block of rows the column sums of the unrounded dz (for the bias).  dz is rounded to T because the matrix
+// cores take T (a second piece would double both products), and pre is kept in T because it is a result's worth of memory between the two
+// passes: 8191 x 1001 x 515 f16 with silu, gradients of x and weight off by 3.0e-4 of their norm, 2.1e-4 with both in f32 (the result's own
+// rounding).  A workgroup takes 256 columns x kSlopeRows rows: 32 threads of eight columns, eight rows at a time.  Bound by the latency of
 // its loads: 8191 x 1001 f16 (49 MB) 20 us with 32 rows a workgroup, 25 with 64; 18 where rows start on 16 bytes.
 constexpr int kSlopeRows = 32;
 template <typename T>
@@ -525,17 +529,20 @@ static bool ready(const void* p, int64_t ld, int64_t cols, int es) {
 
 // Tiles of 256 x 256 (16-bit types, both operands plain, eight waves) where there are enough of them for every compute unit; else four waves on
 // 128 columns x 128, 64 or 32 rows: fewer rows where there are no more, or where that gives no more than three tiles a unit and the sum is too
-// short to be split (up to 32 steps).  The addresses of transposed fragments take too many registers for the largest tile.  Measured in us (128 x 128 / 128 x 64 / 128 x 32):
-//     both transposed (a weight's gradient), f16, 515 x 1001 x 8191, split: 22 / 24 / 32
-//     f32   20 x 3678 x 128    15.5 / 11.0 /  7.4        bf16  20 x 3678 x 128      8.9 /  8.0 /  6.5
-//           1000 x 1000 x 1000 39.4 / 34.8 / 26.6              1000 x 1000 x 1000  20.7 / 20.7 / 10.3
-//           2000 x 2000 x 2048  145 /  140 /  145              2000 x 2000 x 2048  29.6 / 26.5 / 33.2
-//           8192 x 1024 x 2048  262 /  269 /  281              8192 x 1024 x 2048  39.1 / 45.5 / 59.3
-//     and 8192 x 4096 x 4096 bf16 218 with 256 x 256, 315 with 128 x 128.  f32 sums over at most 256 k leave so little to multiply in a tile
-//     that three workgroups a unit hide more of its ends: 5590 x 15976 x 128 with a residual 297 / 278 / 288.
+// short to be split (up to 32 steps).  The addresses of transposed fragments take too many registers for the largest tile.  Measured in us (128 x 128 /
+// 128 x 64 / 128 x 32; f32 from a trace, 16-bit types a call within a graph):
+//     both transposed (a weight's gradient), f16, 512 x 1000 x 8192, split: 26 / 26 / 27
+//     f32   20 x 3678 x 128    15.5 / 11.0 /  7.4        bf16  20 x 3678 x 128      6.2 /  5.6 /  4.5
+//           1000 x 1000 x 1000 39.4 / 34.8 / 26.6              1000 x 1000 x 1000  20.3 / 20.2 / 10.5
+//           2000 x 2000 x 2048  145 /  140 /  145              2000 x 2000 x 2048  30.7 / 27.0 / 37.3
+//           8192 x 1024 x 2048  262 /  269 /  281              8192 x 1024 x 2048  41.1 / 51.6 / 62.4
+//     and 8192 x 4096 x 4096 bf16 228 with 256 x 256, 271 with 128 x 128.  f32 sums over at most 256 k leave so little to multiply in a tile
+//     that three workgroups a unit hide more of its ends (128 / 64 rows): 5590 x 15976 x 128 239 / 224, with a residual 300 / 280, 20000 x 2048 x 64
+//     74 / 68, 8192 x 8192 x 64 117 / 109, x 128 181 / 169, x 200 279 / 265, x 256 297 / 289, 30000 x 1000 x 256 with a residual 165 / 146; beyond that
+//     it fades (8192 x 8192 x 512 541 / 537) and turns (8192 x 1024 x 2048 above).
 // Splits of k for a product with too few tiles to fill 256 compute units: as many as bring it to about two workgroups each, of at least four
-// steps of k.  Measured in us, f32 (bf16), unsplit / two steps / four / eight: 1 x 4096 x 4096 93 / 19.6 / 19.4 / 19.5 (27 / 10.0 / 9.9 / 10.2),
-// 256 x 256 x 4096 265 / 25.8 / 22.9 / 27.1 (37 / 15.0 / 12.4 / 12.9), 700 x 700 x 2100 154 / 41 / 40 / 53 (40 / 27 / 26 / 24); aiming at one or
+// steps of k.  Measured in us, f32 (bf16), unsplit / two steps / four / eight: 1 x 4096 x 4096 93 / 19.6 / 19.4 / 19.5 (33 / 8.8 / 8.7 / 9.5),
+// 256 x 256 x 4096 265 / 25.8 / 22.9 / 27.1 (37 / 14.0 / 11.8 / 12.0), 700 x 700 x 2100 154 / 41 / 40 / 53 (43 / 26 / 25 / 24); aiming at one or
 // four workgroups a unit: 38.7 / 40.4 for the last, 83 / 90 against 83 for 1000 x 500 x 8000.
 struct Shape { int bp, bq, tiles_p, tiles_q, splits, k_split; };
 static Shape shape_of(int64_t np, int64_t nq, int64_t nk, int dtype, bool transposed) {

@@ -88,6 +88,7 @@ __device__ inline void add_scores(SoftmaxState& a, const float* z) {
 // The same with fewer operations: x = fma(z, log2 e, -u) against the rounded u = m log2 e, which drops out when the state is turned into the
 // other form.  Scores beyond 2^126 and, without LEFT_OUT, scores of -inf make s 0 or s or t NaN; the wave then goes through its share again.
 // (4096 x 100003 bf16: 224 us with the other form, of which the vector units were busy 150; 8000 x 13416 f32 with a list 99 against 91.)
+// Off from 64 bits by 1.7e-7 of the results' norm at 8000 x 13416, the same operations one by one in 32 bits by 7e-8.
 struct QuickState {
     float m = -0x1p126f, u = -0x1p126f * kLog2e, s = 0.0f, t = 0.0f;       // u exact: a lane without scores stays 0
     template <int N, bool LEFT_OUT> __device__ inline void add(const float* z) {
